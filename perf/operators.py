@@ -175,7 +175,9 @@ def _table(ctx, new, page, gen, spare, held):
     col = torch.arange(width, device=dev)
     used = int(have.sum())
     table = torch.where(col < have[:, None], order[(start[:, None] + col).clamp(max=n_pages - 1)], torch.full((), -1, dtype=torch.int32, device=dev))
-    return table.contiguous(), order[used:].contiguous(), n_pages
+    # the pages that are left, and room for those that come back
+    free = torch.cat([order[used:], torch.full((used,), -1, dtype=torch.int32, device=dev)])
+    return table.contiguous(), free, n_pages - used
 
 
 def prepare(c, seed):
@@ -200,16 +202,16 @@ def prepare(c, seed):
     page, tokens = c["page"], int(new.sum())
     s.update(ctx=i32(ctx), new=i32(new), tokens=tokens)
     if c["op"] == "plan":
-        table, free, n_pages = _table(ctx, new, page, gen, 37, ctx)
-        # the list of free pages, a count of them, and room below for those that are handed back
-        s.update(table=table, free=free, free_count=i32([free.numel() // (2 if c.get("scarce") else 1)]), n_pages=n_pages, max_tokens=tokens + 5)
+        table, free, left = _table(ctx, new, page, gen, 37, ctx)
+        s.update(table=table, free=free, free_count=i32([left // (2 if c.get("scarce") else 1)]), max_tokens=tokens + 5)
         if own:
             g = s["g"] = _package()
-            s["plan"] = g.KVPlan(c["seqs"], table.shape[1], page, n_pages, tokens + 5)
+            s["plan"] = g.KVPlan(c["seqs"], table.shape[1], page, free.numel(), tokens + 5)
         else:
             s["slots"] = torch.empty(tokens + 5, dtype=torch.int64, device=dev)
         return s
-    table, _, n_pages = _table(ctx, new, page, gen, 3, ctx + new)
+    table, free, _ = _table(ctx, new, page, gen, 3, ctx + new)
+    n_pages = free.numel()
     kvh = c["heads"] if c["op"] == "append" else c["kvh"]
     hd = c["hd"]
     pages = torch.full((n_pages, kvh * page * (hd + 8)), 255, dtype=torch.uint8, device=dev)  # stale: NaN parameters
