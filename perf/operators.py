@@ -211,7 +211,7 @@ def prepare(c, seed):
             s["slots"] = torch.empty(tokens + 5, dtype=torch.int64, device=dev)
         return s
     table, free, _ = _table(ctx, new, page, gen, 3, ctx + new)
-    n_pages = free.numel()
+    n_pages = free.numel() + 1  # the last one belongs to no request
     kvh = c["heads"] if c["op"] == "append" else c["kvh"]
     hd = c["hd"]
     pages = torch.full((n_pages, kvh * page * (hd + 8)), 255, dtype=torch.uint8, device=dev)  # stale: NaN parameters
@@ -322,7 +322,7 @@ def _append(s):
     page, hd, heads = c["page"], c["hd"], c["heads"]
     slots = s["slots"]
     live = slots >= 0
-    # a padded row goes to the last, unused page
+    # a padded row goes to the last page, which nobody reads
     to = torch.where(live, slots, s["pages"].shape[0] * page - 1)
     b = s["pages"].view(-1, heads, page * (hd + 8))
     n = page * hd // 2
