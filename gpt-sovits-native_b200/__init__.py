@@ -140,6 +140,15 @@ SIGNATURES = {
     "gsvk_layernorm_rows": (c_int, [_vp, _vp, _vp, _vp, _sz, _sz, c_double, _vp]),
     "gsvk_softmax_rows": (c_int, [_vp, _vp, _sz, _sz, _vp]),
     "gsvk_activation": (c_int, [_vp, _vp, _sz, c_int, c_float, _vp]),
+    "gsvk_kv_plan": (c_int, [_vp, _vp]),
+    "gsvk_kv_release": (c_int, [_sz, _sz, _sz, c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "gsvk_kv4_page_bytes": (_sz, [c_int, c_int, c_int]),
+    "gsvk_kv4_append": (c_int, [_vp, _vp, _sz, _vp, _sz, c_int, _vp, _sz, _vp]),
+    "gsvk_kv4_read": (c_int, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "gsvk_kv4_attention_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "gsvk_kv4_attention": (c_int, [_vp, _vp]),
+    "gsvk_quantize_rows_i8": (c_int, [_vp, c_int, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
+    "gsvk_gemm_i8": (c_int, [_vp, _vp]),
 }
 
 
@@ -1106,3 +1115,8 @@ class T2SBatch:
             self.close()
         except Exception:
             pass
+
+
+# --------------------------------- quantised serving: 4-bit KV cache, int8 layers
+from .quant import (  # noqa: E402,F401
+    KV4Cache, KV4Workspace, KVPlan, gemm_i8, kv4_page_bytes, quantize_rows_i8)

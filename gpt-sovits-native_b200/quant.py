@@ -1,0 +1,338 @@
+"""Quantised serving: the paged 4-bit KV cache (page plan, append, read back,
+attention) and the 8-bit integer linear layer, over the C ABI of
+include/gsvk.h, which states the value rules and the page layout.
+
+A decode step of many requests is
+
+    plan.run(ctx_len, new_len, table, free, free_count)      # pages and slots, on the GPU
+    for each layer:
+        codes, s = quantize_rows_i8(x)
+        qkv = gemm_i8(codes, s, wqkv, wqkv_scale, bias)
+        cache.append(k, v, plan.slots)
+        y = cache.attention(q, plan.q_start, plan.kv_len, table, scale, max_q, workspace=ws)
+
+Every call is asynchronous on its stream; objects here hold device buffers and
+must not be used from two streams at once.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import byref, c_float, c_int, c_size_t, c_void_p
+
+from . import ACT_NONE, _stream, check, lib
+
+_vp, _sz = c_void_p, c_size_t
+
+
+class KVPlanArgs(ctypes.Structure):
+    _fields_ = [("n_seq", _sz), ("max_blocks", _sz), ("n_pages", _sz), ("max_tokens", _sz),
+                ("page_size", c_int), ("ctx_len", _vp), ("new_len", _vp), ("block_table", _vp),
+                ("free_pages", _vp), ("free_count", _vp), ("q_start", _vp), ("kv_len", _vp),
+                ("slots", _vp), ("free_left", _vp), ("refused", _vp), ("workspace", _vp)]
+
+
+class KV4CacheArgs(ctypes.Structure):
+    _fields_ = [("pages", _vp), ("n_pages", _sz), ("page_size", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int)]
+
+
+class KV4AttentionArgs(ctypes.Structure):
+    _fields_ = [("cache", KV4CacheArgs), ("q", _vp), ("q_stride", _sz), ("out", _vp),
+                ("out_stride", _sz), ("heads", _sz), ("n_tokens", _sz), ("n_seq", _sz),
+                ("max_blocks", _sz), ("max_q", _sz), ("q_start", _vp), ("kv_len", _vp),
+                ("prefix", _vp), ("block_table", _vp), ("scale", c_float), ("workspace", _vp),
+                ("workspace_bytes", _sz)]
+
+
+class GemmI8Args(ctypes.Structure):
+    _fields_ = [("a", _vp), ("lda", _sz), ("b", _vp), ("ldb", _sz), ("a_scale", _vp),
+                ("b_scale", _vp), ("M", _sz), ("N", _sz), ("K", _sz), ("bias", _vp),
+                ("residual", _vp), ("ld_res", _sz), ("c", _vp), ("ldc", _sz), ("c_f16", _vp),
+                ("ldc_f16", _sz), ("act", c_int), ("slope", c_float)]
+
+
+def _tensor(t, dtype, what, dim=None):
+    """A CUDA tensor of one type whose rows are contiguous; its address."""
+    if not t.is_cuda:
+        raise ValueError(f"{what}: gsvk takes CUDA tensors")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {dtype} expected, got {t.dtype}")
+    if dim is not None and t.dim() != dim:
+        raise ValueError(f"{what}: {dim} dimensions expected, got {t.dim()}")
+    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: gsvk takes tensors with unit inner stride")
+    return t.data_ptr()
+
+
+def _vector(t, dtype, n, what):
+    """Address of a contiguous vector of at least n values."""
+    p = _tensor(t, dtype, what)
+    if t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous values expected")
+    return p
+
+
+def _row_stride(t):
+    """Elements between the rows of a 2-D tensor (one row: any)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows(t, dtype, heads, head_dim, what):
+    """Address and row stride of [tokens, heads, head_dim] rows whose heads lie side by side."""
+    p = _tensor(t, dtype, what, 3)
+    if t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ValueError(f"{what}: [tokens, {heads}, {head_dim}] expected, got {tuple(t.shape)}")
+    if heads > 1 and t.stride(1) != head_dim:
+        raise ValueError(f"{what}: the heads of a row lie side by side")
+    return p, t.stride(0) if t.shape[0] > 1 else heads * head_dim
+
+
+def _new(shape, dtype, device, stream):
+    """An output of this call, kept by the allocator until `stream` is done with it."""
+    import torch
+
+    t = torch.empty(shape, dtype=dtype, device=device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+# ------------------------------------------------------------------ page plan
+class KVPlan:
+    """Pages and slots of each step of up to `n_seq` requests, built on the GPU
+    (gsvk_kv_plan).  Holds the results: q_start, kv_len, slots, free_left,
+    refused."""
+
+    def __init__(self, n_seq: int, max_blocks: int, page_size: int, n_pages: int, max_tokens: int,
+                 device=None):
+        import torch
+
+        device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        i32 = dict(dtype=torch.int32, device=device)
+        self.n_seq, self.max_blocks, self.n_pages = int(n_seq), int(max_blocks), int(n_pages)
+        self.page_size, self.max_tokens = int(page_size), int(max_tokens)
+        self.q_start = torch.zeros(n_seq + 1, **i32)
+        self.kv_len = torch.zeros(n_seq, **i32)
+        self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
+        self.free_left = torch.zeros(1, **i32)
+        self.refused = torch.zeros(1, **i32)
+        self._ticket = torch.zeros(1, **i32)
+        self._args = KVPlanArgs(
+            n_seq=self.n_seq, max_blocks=self.max_blocks, n_pages=self.n_pages,
+            max_tokens=self.max_tokens, page_size=self.page_size, q_start=self.q_start.data_ptr(),
+            slots=self.slots.data_ptr(), refused=self.refused.data_ptr(),
+            workspace=self._ticket.data_ptr())
+
+    def _state(self, length, block_table, free_pages, free_count):
+        import torch
+
+        i32 = torch.int32
+        if tuple(block_table.shape) != (self.n_seq, self.max_blocks):
+            raise ValueError(f"block_table: {(self.n_seq, self.max_blocks)} expected, got "
+                             f"{tuple(block_table.shape)}")
+        return (_vector(length, i32, self.n_seq, "lengths"),
+                _vector(block_table, i32, 0, "block_table"),
+                _vector(free_pages, i32, self.n_pages, "free_pages"),
+                _vector(free_count, i32, 1, "free_count"))
+
+    def run(self, ctx_len, new_len, block_table, free_pages, free_count, in_place=False,
+            stream=None):
+        """Plans one step: `ctx_len` cached and `new_len` new tokens of each
+        request (int32), the block table [n_seq, max_blocks], and the pool's
+        free_pages[: free_count].  in_place: ctx_len and free_count become the
+        lengths and the count after the step (and stand for kv_len and
+        free_left), else those go to this object's own."""
+        import torch
+
+        a = self._args
+        a.ctx_len, a.block_table, a.free_pages, a.free_count = self._state(
+            ctx_len, block_table, free_pages, free_count)
+        a.new_len = _vector(new_len, torch.int32, self.n_seq, "new_len")
+        a.kv_len = a.ctx_len if in_place else self.kv_len.data_ptr()
+        a.free_left = a.free_count if in_place else self.free_left.data_ptr()
+        check(lib().gsvk_kv_plan(byref(a), _stream(stream)))
+        return self
+
+    def release(self, done, length, block_table, free_pages, free_count, stream=None):
+        """Returns the pages of the requests with done != 0 to the pool (in place)."""
+        import torch
+
+        ln, table, free, count = self._state(length, block_table, free_pages, free_count)
+        check(lib().gsvk_kv_release(self.n_seq, self.max_blocks, self.n_pages, self.page_size,
+                                    _vector(done, torch.int32, self.n_seq, "done"), ln, table, free,
+                                    count, _stream(stream)))
+
+
+# ------------------------------------------------------------- 4-bit KV cache
+def kv4_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of a page; 0 where the sizes are not supported."""
+    return lib().gsvk_kv4_page_bytes(page_size, kv_heads, head_dim)
+
+
+class KV4Workspace:
+    """Scratch of KV4Cache.attention for up to `n_seq` requests and `n_tokens`
+    rows; the layers of a model share one."""
+
+    def __init__(self, n_seq: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int,
+                 device=None):
+        import torch
+
+        self.bytes = lib().gsvk_kv4_attention_workspace(n_seq, n_tokens, heads, kv_heads, head_dim)
+        if self.bytes == 0:
+            raise ValueError(f"no attention for {n_seq} requests, {n_tokens} rows, {heads} heads "
+                             f"over {kv_heads} of {head_dim}")
+        device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.buffer = torch.zeros(self.bytes, dtype=torch.uint8, device=device)
+        self.ptr = self.buffer.data_ptr()
+
+
+class KV4Cache:
+    """One layer's pages: a uint8 CUDA tensor [n_pages, kv4_page_bytes(...)]."""
+
+    def __init__(self, pages, page_size: int, kv_heads: int, head_dim: int):
+        import torch
+
+        size = kv4_page_bytes(page_size, kv_heads, head_dim)
+        if size == 0:
+            raise ValueError(f"no 4-bit cache with pages of {page_size} tokens, {kv_heads} heads "
+                             f"of {head_dim}")
+        p = _vector(pages, torch.uint8, size, "pages")
+        if pages.numel() % size:
+            raise ValueError(f"pages: whole pages of {size} bytes expected")
+        self.pages = pages
+        self.page_size, self.kv_heads, self.head_dim = int(page_size), int(kv_heads), int(head_dim)
+        self.n_pages = pages.numel() // size
+        self._cache = KV4CacheArgs(p, self.n_pages, self.page_size, self.kv_heads, self.head_dim)
+        self._attn = KV4AttentionArgs(cache=self._cache)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None):
+        import torch
+
+        size = kv4_page_bytes(page_size, kv_heads, head_dim)
+        device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        return cls(torch.empty(n_pages, max(size, 1), dtype=torch.uint8, device=device), page_size,
+                   kv_heads, head_dim)
+
+    def append(self, k, v, slots, stream=None):
+        """Quantises rows [tokens, kv_heads, head_dim] (fp16 or fp32) into their
+        slots (int64; those outside the cache, such as -1, are skipped)."""
+        import torch
+
+        kp, ks = _rows(k, v.dtype, self.kv_heads, self.head_dim, "k")
+        vp, vs = _rows(v, v.dtype, self.kv_heads, self.head_dim, "v")
+        if v.dtype not in (torch.float16, torch.float32):
+            raise TypeError(f"k, v: fp16 or fp32 expected, got {v.dtype}")
+        n = k.shape[0]
+        if v.shape[0] != n:
+            raise ValueError(f"k, v: {n} and {v.shape[0]} rows")
+        check(lib().gsvk_kv4_append(byref(self._cache), kp, ks, vp, vs, v.dtype == torch.float32,
+                                    _vector(slots, torch.int64, n, "slots"), n, _stream(stream)))
+
+    def read(self, slots, k=None, v=None, stream=None):
+        """What the slots stand for: fp16 rows k and v [len(slots), kv_heads,
+        head_dim], zeros for a slot outside the cache."""
+        import torch
+
+        n = slots.numel()
+        shape = (n, self.kv_heads, self.head_dim)
+        if k is None and v is None:
+            k, v = (_new(shape, torch.float16, slots.device, stream) for _ in range(2))
+        ptrs = []
+        for t, what in ((k, "k"), (v, "v")):
+            if t is not None and t.shape[0] != n:
+                raise ValueError(f"{what}: {n} rows expected, got {t.shape[0]}")
+            ptrs += _rows(t, torch.float16, self.kv_heads, self.head_dim, what) if t is not None \
+                else (None, 0)
+        check(lib().gsvk_kv4_read(byref(self._cache), _vector(slots, torch.int64, n, "slots"), n,
+                                  *ptrs, _stream(stream)))
+        return k, v
+
+    def attention(self, q, q_start, kv_len, block_table, scale: float, max_q: int, workspace,
+                  prefix=None, out=None, stream=None):
+        """Attention of packed rows q [tokens, heads, head_dim] (fp16) over the
+        cache (gsvk_kv4_attention): request i owns rows q_start[i] to
+        q_start[i + 1], sees kv_len[i] keys causally from the end and its
+        first prefix[i] from every row.  `workspace`: a KV4Workspace of at
+        least these sizes.  Returns fp16 rows like q."""
+        import torch
+
+        i32 = torch.int32
+        if q.dim() != 3:
+            raise ValueError(f"q: [tokens, heads, {self.head_dim}] expected, got {tuple(q.shape)}")
+        n, heads = q.shape[0], q.shape[1]
+        a = self._attn
+        a.q, a.q_stride = _rows(q, torch.float16, heads, self.head_dim, "q")
+        if out is None:
+            out = _new(q.shape, torch.float16, q.device, stream)
+        elif out.shape != q.shape:
+            raise ValueError(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
+        a.out, a.out_stride = _rows(out, torch.float16, heads, self.head_dim, "out")
+        _tensor(block_table, i32, "block_table", 2)
+        n_seq = block_table.shape[0]
+        a.heads, a.n_tokens, a.n_seq, a.max_blocks = heads, n, n_seq, block_table.shape[1]
+        a.max_q, a.scale = max_q, scale
+        a.q_start = _vector(q_start, i32, n_seq + 1, "q_start")
+        a.kv_len = _vector(kv_len, i32, n_seq, "kv_len")
+        a.prefix = _vector(prefix, i32, n_seq, "prefix") if prefix is not None else None
+        a.block_table = _vector(block_table, i32, 0, "block_table")
+        a.workspace, a.workspace_bytes = workspace.ptr, workspace.bytes
+        check(lib().gsvk_kv4_attention(byref(a), _stream(stream)))
+        return out
+
+
+# -------------------------------------------------------- 8-bit linear layers
+def quantize_rows_i8(x, q=None, scale=None, stream=None):
+    """Rows of x [rows, n] (fp16 or fp32) as int8 codes and an fp32 scale each.
+    A new q has its rows in whole 16 bytes, as gemm_i8's tensor-core path
+    takes them."""
+    import torch
+
+    if x.dtype not in (torch.float16, torch.float32):
+        raise TypeError(f"x: fp16 or fp32 expected, got {x.dtype}")
+    xp = _tensor(x, x.dtype, "x", 2)
+    rows, n = x.shape
+    if q is None:
+        q = _new((rows, (n + 15) & ~15), torch.int8, x.device, stream)[:, :n]
+    elif tuple(q.shape) != (rows, n):
+        raise ValueError(f"q: {(rows, n)} expected, got {tuple(q.shape)}")
+    if scale is None:
+        scale = _new((rows,), torch.float32, x.device, stream)
+    check(lib().gsvk_quantize_rows_i8(xp, x.dtype == torch.float32, rows, n, _row_stride(x),
+                                      _tensor(q, torch.int8, "q", 2),
+                                      q.stride(0) if rows > 1 else n,
+                                      _vector(scale, torch.float32, rows, "scale"),
+                                      _stream(stream)))
+    return q, scale
+
+
+def gemm_i8(a, a_scale, b, b_scale, bias=None, residual=None, act=ACT_NONE, slope=0.0, c=None,
+            c_f16=None, stream=None):
+    """act(a_scale[m] b_scale[n] sum_k a[m, k] b[n, k] + bias) + residual: int8
+    a [M, K] and b [N, K] -> fp32 c and / or fp16 c_f16 (a new fp16 one
+    where neither is given)."""
+    import torch
+
+    ap, bp = _tensor(a, torch.int8, "a", 2), _tensor(b, torch.int8, "b", 2)
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K:
+        raise ValueError(f"a, b: rows of {K} and {b.shape[1]}")
+    if c is None and c_f16 is None:
+        c_f16 = _new((M, N), torch.float16, a.device, stream)
+    f32 = torch.float32
+    for t, dt, what in ((c, f32, "c"), (c_f16, torch.float16, "c_f16"), (residual, f32, "residual")):
+        if t is not None:
+            _tensor(t, dt, what, 2)
+            if t.shape[0] != M or t.shape[1] != N:
+                raise ValueError(f"{what}: {(M, N)} expected, got {tuple(t.shape)}")
+    g = GemmI8Args(ap, a.stride(0) if M > 1 else K, bp, b.stride(0) if N > 1 else K,
+                   _vector(a_scale, f32, M, "a_scale"), _vector(b_scale, f32, N, "b_scale"), M, N, K,
+                   None if bias is None else _vector(bias, f32, N, "bias"),
+                   None if residual is None else residual.data_ptr(),
+                   0 if residual is None else _row_stride(residual),
+                   None if c is None else c.data_ptr(), 0 if c is None else _row_stride(c),
+                   None if c_f16 is None else c_f16.data_ptr(),
+                   0 if c_f16 is None else _row_stride(c_f16), act, slope)
+    check(lib().gsvk_gemm_i8(byref(g), _stream(stream)))
+    return c if c is not None else c_f16

@@ -649,6 +649,168 @@ int gsvk_t2s_batch_launches_per_step(gsvk_t2s_batch_t h);
 int gsvk_t2s_batch_set_attention(gsvk_t2s_batch_t h, int kind);
 int gsvk_t2s_batch_attention(gsvk_t2s_batch_t h);
 
+/* ---- paged 4-bit KV cache ----------------------------------------------- */
+/* A cache of pages for requests of any length, K and V held in 4 bits.  No
+ * counterpart in the reference, whose cache is one dense fp16 buffer per
+ * request (t2s_engine.hpp:129-131); a page of this cache takes
+ * (head_dim + 8) / (4 head_dim) of the same tokens' fp16 rows (0.31 at head_dim 32, 0.27
+ * at 128) and requests share one pool of pages.
+ *
+ * Values.  A row x (one token, one kv head, K or V) is held as 16 levels
+ * between its least and greatest value:
+ *   low = fp16(min x), step = fp16((max x - min x) / 15),
+ *   code_d = clamp(rint((x_d - low) / step), 0, 15)   (0 where step is 0),
+ * and stands for step * code_d + low.  Arithmetic in fp32, IEEE division,
+ * round to nearest even.  A row with a NaN, an infinity or a magnitude that
+ * fp16 cannot hold stands for NaN throughout, and only that row.
+ *
+ * Layout.  Page p starts at pages + p * gsvk_kv4_page_bytes(...).  For each
+ * kv head in turn it holds
+ *   K codes  [page_size][head_dim / 2] bytes, dimension 2i in the low and
+ *            2i + 1 in the high nibble of byte i,
+ *   V codes  likewise,
+ *   K parameters [page_size][2] fp16: step, low,
+ *   V parameters likewise.
+ * The token at position t of a request is row t % page_size of the page
+ * block_table[t / page_size]; its slot is page * page_size + t % page_size.
+ * Calls with no rows do nothing and take any pointers. */
+typedef struct {
+  uint8_t* pages;    /* DEVICE, 16-byte aligned, n_pages * page bytes */
+  size_t n_pages;    /* below 2^31 */
+  int page_size;     /* tokens: 16, 32, 64 or 128 */
+  int kv_heads;      /* 1 .. 1024 */
+  int head_dim;      /* 32, 64 or 128 */
+} gsvk_kv4_cache;
+/* Bytes of one page, a multiple of 128; 0 where the sizes are not supported. */
+size_t gsvk_kv4_page_bytes(int page_size, int kv_heads, int head_dim);
+
+/* Page plan of one step, built on the device from the requests' lengths (no
+ * length visits the host).  All pointers DEVICE.  Request i has ctx_len[i]
+ * tokens cached and adds new_len[i] (0 for one that rests).  It needs
+ *   need_i = ceil((ctx_i + new_i) / page_size) - ceil(ctx_i / page_size)
+ * pages more and is granted them when need_i is 0 or the sum of need over
+ * requests 0 .. i is at most *free_count; pages come off the end of
+ * free_pages[0 .. *free_count) in the requests' order.  A request that is not
+ * granted, whose length is negative, passes max_blocks pages or whose tokens end past
+ * max_tokens is refused: it keeps its pages and its length (the latter kinds need no
+ * pages in the sum above).  Results:
+ *   q_start[n_seq + 1]   first row of each request in the step's packed rows
+ *                        (refused ones included; a negative new_len counts as 0)
+ *   kv_len[n_seq]        tokens cached after the step: ctx + new, or ctx where refused
+ *   block_table          [n_seq][max_blocks], entries of the granted pages written
+ *   slots[max_tokens]    slot of each packed row; -1 for refused rows and past the last
+ *   free_left[1], refused[1]   pages left, requests refused
+ * kv_len may be ctx_len and free_left may be free_count (a step in place);
+ * otherwise the inputs are left as they are and a second call gives the same.
+ * workspace: one int32, zero before the first call and left zero by each. */
+typedef struct {
+  size_t n_seq;       /* 1 .. 16384 */
+  size_t max_blocks;  /* columns of block_table */
+  size_t n_pages;     /* pages of the pool = entries of free_pages */
+  size_t max_tokens;  /* entries of slots */
+  int page_size;
+  const int32_t* ctx_len;
+  const int32_t* new_len;
+  int32_t* block_table;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* q_start;
+  int32_t* kv_len;
+  int64_t* slots;
+  int32_t* free_left;
+  int32_t* refused;
+  int32_t* workspace;
+} gsvk_kv_plan_args;
+int gsvk_kv_plan(const gsvk_kv_plan_args* args, gsvk_stream_t stream);
+/* Takes back the pages of every request with done[i] != 0: the first
+ * ceil(len_i / page_size) entries of its block_table row are appended to
+ * free_pages in the requests' order (entries outside [0, n_pages) stay out),
+ * *free_count grows by as many, the entries become -1 and len[i] becomes 0.
+ * Nothing past entry n_pages - 1 of free_pages is written.  DEVICE pointers. */
+int gsvk_kv_release(size_t n_seq, size_t max_blocks, size_t n_pages, int page_size,
+                    const int32_t* done, int32_t* len, int32_t* block_table, int32_t* free_pages,
+                    int32_t* free_count, gsvk_stream_t stream);
+
+/* Quantises n_tokens rows of K and V into their slots (DEVICE int64; a slot
+ * outside the cache, such as -1, is skipped).  Row t of K starts at
+ * k + t * k_stride elements and holds its heads side by side; fp32 rows when
+ * is_f32, else fp16 bits.  Pointers and strides in whole 16 bytes.  Two rows
+ * of one call must not have the same slot. */
+int gsvk_kv4_append(const gsvk_kv4_cache* cache, const void* k, size_t k_stride, const void* v,
+                    size_t v_stride, int is_f32, const int64_t* slots, size_t n_tokens,
+                    gsvk_stream_t stream);
+/* What the slots stand for, rounded to fp16 once (within its finite range): rows [n_tokens] of k and v
+ * with their own strides (k or v may be NULL); zeros for a slot outside the cache. */
+int gsvk_kv4_read(const gsvk_kv4_cache* cache, const int64_t* slots, size_t n_tokens, uint16_t* k,
+                  size_t k_stride, uint16_t* v, size_t v_stride, gsvk_stream_t stream);
+
+/* Attention of a step's packed rows over the cache.  Request i owns rows
+ * q_start[i] .. q_start[i+1) of q and out (fp16; query head a at column
+ * a * head_dim, reading kv head a / (heads / kv_heads)); its row r sees keys
+ * j < limit,
+ *   limit = min(kv_len_i, max(prefix_i, kv_len_i - n_i + r + 1)),  n_i its rows:
+ * causal with the last row on the last key, and with `prefix` (NULL: 0) the
+ * first prefix_i keys seen by every row, as in the T2S prefill
+ * (t2s_engine.cpp:881-1034).  out = softmax(scale q.k) . v over those keys,
+ * zeros where there is none.  Scores, statistics and sums are fp32, the
+ * result is rounded to fp16 once.  Keys past the limit are not read into the
+ * result, whatever their page holds; entries of block_table outside
+ * [0, n_pages) count as keys past the limit.  Rows outside every
+ * request are left as they are.  max_q: a bound on the longest request's rows, for
+ * the choice of kernel (results hold for any value).
+ * workspace: DEVICE, 256-byte aligned, gsvk_kv4_attention_workspace() bytes, zero before the
+ * first call and left so; calls that may overlap need one each. */
+typedef struct {
+  gsvk_kv4_cache cache;
+  const uint16_t* q; size_t q_stride;     /* elements between rows, a multiple of 8 */
+  uint16_t* out; size_t out_stride;
+  size_t heads;                           /* a multiple of kv_heads */
+  size_t n_tokens;                        /* rows of q and out */
+  size_t n_seq;                           /* 1 .. 16384 */
+  size_t max_blocks;                      /* columns of block_table */
+  size_t max_q;
+  const int32_t* q_start;                 /* [n_seq + 1], ascending from 0 to at most n_tokens */
+  const int32_t* kv_len;                  /* [n_seq] */
+  const int32_t* prefix;                  /* [n_seq] or NULL */
+  const int32_t* block_table;             /* [n_seq][max_blocks] */
+  float scale;
+  void* workspace; size_t workspace_bytes;
+} gsvk_kv4_attention_args;
+/* Bytes for calls of up to n_seq requests and n_tokens rows; 0 where the sizes
+ * are not supported. */
+size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads, size_t kv_heads,
+                                    size_t head_dim);
+int gsvk_kv4_attention(const gsvk_kv4_attention_args* args, gsvk_stream_t stream);
+
+/* ---- 8-bit integer products --------------------------------------------- */
+/* Row quantiser for gsvk_gemm_i8, for activations (per token) and weights
+ * (per output channel): scale = max |x| / 127, q = rint(x / scale) (0 where
+ * the scale is 0), fp32 arithmetic with IEEE division.  A row with a NaN or
+ * an infinity gets q = 0 and scale = NaN.  x: fp32 when is_f32, else fp16 bits, rows
+ * ldx elements apart (0: n); q rows ldq bytes apart (0: n), scale fp32 [rows].
+ * Columns n .. ldq of a row are left as they are. */
+int gsvk_quantize_rows_i8(const void* x, int is_f32, size_t rows, size_t n, size_t ldx, int8_t* q,
+                          size_t ldq, float* scale, gsvk_stream_t stream);
+/* C[m, n] = act(a_scale[m] b_scale[n] sum_k A[m, k] B[n, k] + bias[n]) + residual[m, n]:
+ * int8 operands, exact 32-bit sums (K below 131072), fp32 epilogue, written as fp32
+ * and/or fp16.  Leading dimensions of 0 mean dense rows.  Operands that are
+ * 16-byte aligned with leading dimensions in whole 16 bytes run on the
+ * tensor cores (any K: what lies between K and the leading dimension is not
+ * read), others on a CUDA-core kernel with the same results. */
+typedef struct {
+  const int8_t* a; size_t lda;       /* [M, K] */
+  const int8_t* b; size_t ldb;       /* [N, K] */
+  const float* a_scale;              /* [M] */
+  const float* b_scale;              /* [N] */
+  size_t M, N, K;
+  const float* bias;                 /* [N] or NULL */
+  const float* residual; size_t ld_res; /* fp32 [M, N] or NULL; may be c itself */
+  float* c; size_t ldc;              /* fp32 output or NULL */
+  uint16_t* c_f16; size_t ldc_f16;   /* fp16 output or NULL */
+  int act; float slope;              /* GSVK_ACT_* */
+} gsvk_gemm_i8_args;
+int gsvk_gemm_i8(const gsvk_gemm_i8_args* args, gsvk_stream_t stream);
+
 /* ---- T2S inspection (synchronous reads of the batch-1 engine) ----------- */
 /* The logits the last step sampled from (raw, before the penalty); synchronous. */
 int gsvk_t2s_read_logits(gsvk_t2s_t h, float* host_out);
