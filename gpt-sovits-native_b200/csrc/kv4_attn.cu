@@ -3,6 +3,7 @@
 
 #include "gsvk_internal.hpp"
 #include "kv4.cuh"
+#include "tma.cuh"
 
 namespace gsvk {
 
@@ -22,87 +23,686 @@ struct AttnArgs {
   const int32_t* prefix;
   const int32_t* table;
   float scale_log2;  // scale * log2(e)
+  int* tickets;      // of the items that several warps share
+  float* parts;      // their records
+  uint32_t* status;
 };
 
-constexpr int kSimpleWarps = 4;
+// ------------------------------------------------------------ few query rows
+// Work.  An item is (request, kv head, block of up to ROWS query rows), a row
+// being one (new token, query head of the group); its unit of work is a tile
+// of 64 keys.  The units of all items lie on one line (request, head, block,
+// tile), which is cut into equal runs, one per warp of the grid, so ragged
+// lengths leave no warp idle and a single long request fills the GPU.  Every
+// CTA works the line out for itself from the lengths (a block-wide sum over
+// the requests).  An item cut between warps is joined by the warp that
+// arrives last, in the order of the runs, so results do not depend on timing.
+//
+// Data.  A tile is one contiguous block per page and head; a lane per page
+// copies it with cp.async.bulk into its warp's own ring of shared memory,
+// several tiles ahead.  Warps never wait for one another.
+//
+// Mathematics.  With k_j = a_j c_j + b_j (step, codes, low) the score is
+//   q.k_j = a_j (q.c_j) + b_j sum(q),
+// and sum_j p_j v_j = sum_j (p_j a_j) c_j + sum_j p_j b_j, so both products run
+// on the tensor cores (m16n8k16, fp32 sums) over the codes alone.  A nibble
+// pair masked out of a word, (w >> s) & 0x000f000f, is a pair of fp16
+// subnormals worth c 2^-24, which the tensor cores multiply exactly; the
+// nibbles at bits 4 and 20 are worth 16 c 2^-24 and have sums of their own.
+// So a code costs 5/8 of an instruction to unpack for the scores, and 3/4 for
+// the values, where two tokens' words are first interleaved by prmt.
+// The weights p_j a_j, scaled by a power of two so that the greatest step seen is
+// at most 1, go in as two fp16 parts, whose sum holds 22 bits: with
+// ROWS = 8 the second part takes the unused rows 8..15 of the same MMA.
+constexpr int kTile = 64;          // keys of a unit
+constexpr int kSplitWarps = 4;     // warps of a CTA
+constexpr int kMaxPieces = 64;     // warps that share an item
 
-// One warp per (row, query head): 32 keys at a time, a lane to a key for the
-// scores and to head_dim / 32 dimensions for the sums.
 template <int HD>
-__global__ void __launch_bounds__(kSimpleWarps * 32) kv4_attn_rows_kernel(const AttnArgs a) {
-  __shared__ float s_q[kSimpleWarps][HD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * kSimpleWarps + warp;
-  if (item >= static_cast<long long>(a.n_tokens) * a.heads) return;
-  const int t = static_cast<int>(item / a.heads), head = static_cast<int>(item % a.heads);
-  int lo = 0, hi = a.n_seq + 1;  // the last request starting at or before t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.q_start[mid] <= t) {
-      lo = mid;
-    } else {
-      hi = mid;
-    }
-  }
-  if (lo >= a.n_seq || t < a.q_start[0]) return;  // a row of no request
-  const int len = a.kv_len[lo], n = a.q_start[lo + 1] - a.q_start[lo];
-  int limit = len - n + (t - a.q_start[lo]) + 1;
-  if (a.prefix) limit = max(limit, a.prefix[lo]);
-  limit = max(0, min(limit, min(len, a.max_blocks << a.shift)));
-  const uint16_t* q = a.q + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(head) * HD;
-  float qsum = 0.f;
-  for (int d = lane; d < HD; d += 32) {
-    const float x = h2f(q[d]);
-    s_q[warp][d] = x;
-    qsum += x;
-  }
-  qsum = warp_sum(qsum);
-  __syncwarp();
-  const size_t head_off = static_cast<size_t>(head / a.group) * kv4_head_bytes(a.shift, HD);
-  const int32_t* row = a.table + static_cast<size_t>(lo) * a.max_blocks;
-  float m = -INFINITY, l = 0.f, acc[HD / 32] = {};
-  for (int j0 = 0; j0 < limit; j0 += 32) {
-    const int j = j0 + lane;
-    const int page = j < limit ? row[j >> a.shift] : -1;
-    const bool live = page >= 0 && page < a.n_pages;
-    const uint8_t* b = a.pages + static_cast<size_t>(live ? page : 0) * a.page_bytes + head_off;
-    const int at = j & ((1 << a.shift) - 1);
-    float s = -INFINITY;
-    uint32_t vp = 0;
-    if (live) {
-      float dot = 0.f;
-      for (int i = 0; i < HD / 8; ++i) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(b + at * (HD / 2) + i * 4);
-        for (int u = 0; u < 8; ++u) dot = fmaf(s_q[warp][8 * i + u], float((w >> (4 * u)) & 15u), dot);
-      }
-      const uint32_t kp = *reinterpret_cast<const uint32_t*>(b + kv4_k_par(a.shift, HD) + at * 4);
-      vp = *reinterpret_cast<const uint32_t*>(b + kv4_v_par(a.shift, HD) + at * 4);
-      s = fmaf(h2f(uint16_t(kp)), dot, h2f(uint16_t(kp >> 16)) * qsum) * a.scale_log2;
-    }
-    const float mn = fmaxf(m, warp_max(s));
-    const float ref = mn == -INFINITY ? 0.f : mn;  // no key seen yet
-    const float keep = exp2f(m - ref), p = exp2f(s - ref);
-    m = mn;
-    l = fmaf(l, keep, p);
-    for (int i = 0; i < HD / 32; ++i) acc[i] *= keep;
-    for (int u = 0; u < 32; ++u) {
-      const float pu = __shfl_sync(0xffffffffu, p, u);
-      const uint32_t par = __shfl_sync(0xffffffffu, vp, u);
-      const unsigned long long bu = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(b), u);
-      const int pos = (j0 + u) & ((1 << a.shift) - 1);
-      if (pu == 0.f) continue;
-      const uint8_t* c = reinterpret_cast<const uint8_t*>(bu) + kv4_v_codes(a.shift, HD) + pos * (HD / 2);
-      for (int i = 0; i < HD / 32; ++i) {
-        const int d = lane + 32 * i;
-        const float code = float((c[d >> 1] >> (4 * (d & 1))) & 15);
-        acc[i] = fmaf(pu, fmaf(h2f(uint16_t(par)), code, h2f(uint16_t(par >> 16))), acc[i]);
-      }
-    }
-  }
-  l = warp_sum(l);
-  uint16_t* o = a.out + static_cast<size_t>(t) * a.out_stride + static_cast<size_t>(head) * HD;
-  for (int i = 0; i < HD / 32; ++i) o[lane + 32 * i] = f2h(l > 0.f || l != l ? acc[i] / l : 0.f);
+constexpr int kStages = HD == 32 ? 4 : 3;
+template <int HD>
+constexpr int kCtasPerSm = HD == 128 ? 2 : HD == 64 ? 3 : 4;
+template <int HD>
+constexpr int kTileBytes = kTile * (HD + 8);
+template <int HD>
+constexpr int kRecord = HD + 4;  // floats of a joined row: maximum, sum, (pad), values
+
+// One request's rows and the keys they see.
+struct Request {
+  int q0, n, len, prefix;
+};
+__device__ __forceinline__ Request request_of(const AttnArgs& a, int s) {
+  Request r;
+  r.q0 = a.q_start[s];
+  r.n = min(a.q_start[s + 1], a.n_tokens) - r.q0;
+  if (r.q0 < 0) r.n = 0;
+  r.len = a.kv_len[s];
+  r.prefix = a.prefix ? a.prefix[s] : 0;
+  return r;
 }
+// Keys that row r of a request sees (64-bit on the way: lengths are the caller's).
+__device__ __forceinline__ int limit_of(const AttnArgs& a, const Request& q, int r) {
+  const long long causal = static_cast<long long>(q.len) - q.n + r + 1;
+  const long long see = max(causal, static_cast<long long>(q.prefix));
+  const long long have = min(q.len, a.max_blocks << a.shift);
+  return static_cast<int>(max(0LL, min(see, have)));
+}
+template <int ROWS>
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Request& q, int block) {
+  const int last = min((block + 1) * ROWS, q.n * a.group) - 1;
+  return max(1, (limit_of(a, q, last / a.group) + kTile - 1) / kTile);
+}
+template <int ROWS>
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, const Request& q) {
+  return q.n > 0 ? (q.n * a.group + ROWS - 1) / ROWS : 0;
+}
+// Units of one kv head of a request; *most keeps the longest item.
+template <int ROWS>
+__device__ __forceinline__ long long head_units(const AttnArgs& a, const Request& q, int* most) {
+  long long u = 0;
+  const int nb = blocks_of<ROWS>(a, q);
+  for (int b = 0; b < nb; ++b) {
+    const int t = tiles_of<ROWS>(a, q, b);
+    u += t;
+    *most = max(*most, t);
+  }
+  return u;
+}
+
+// A place on the line of units.
+template <int ROWS>
+struct Cursor {
+  Request req;
+  int seq, head, block, tile, tiles, blocks;
+
+  __device__ void enter(const AttnArgs& a, int s, int h, int b) {
+    seq = s;
+    req = request_of(a, s);
+    blocks = blocks_of<ROWS>(a, req);
+    head = h;
+    block = b;
+    tile = 0;
+    tiles = blocks > 0 ? tiles_of<ROWS>(a, req, b) : 0;
+  }
+  __device__ void next_item(const AttnArgs& a) {
+    tile = 0;
+    if (++block < blocks) {
+      tiles = tiles_of<ROWS>(a, req, block);
+      return;
+    }
+    block = 0;
+    if (++head < a.kv_heads) {
+      if (blocks > 1) tiles = tiles_of<ROWS>(a, req, 0);
+      return;
+    }
+    int s = seq + 1;
+    do {
+      enter(a, min(s, a.n_seq - 1), 0, 0);
+    } while (blocks == 0 && ++s < a.n_seq);
+  }
+};
+
+__device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two weights as fp16, and what that rounding left.
+__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = f2h2(x - f.x, y - f.y);
+}
+
+// The state of ROWS query rows over the tiles seen so far.  Lane (g, t) = (lane / 4, lane % 4) has row g
+// (ROWS = 16: and row g + 8); its part of the sums o is head_dim / 4 dimensions from t head_dim / 4 on.
+template <int HD, int ROWS>
+struct RowState {
+  static constexpr int kR = ROWS / 8;
+  uint32_t q[HD / 32][2][2 * kR];  // [word][even, odd nibbles][A registers]
+  float o[HD / 8][4];
+  float m[kR], l[kR], pb[kR], qsum[kR];
+  float unit;  // weights are held in this power of two
+};
+
+template <int HD, int ROWS>
+__device__ __forceinline__ void load_rows(const AttnArgs& a, const Request& rq, int head, int block, int lane,
+                                          RowState<HD, ROWS>& s) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int k = 0; k < RowState<HD, ROWS>::kR; ++k) {
+    const int row = block * ROWS + 8 * k + g;
+    const bool ok = row < rq.n * a.group;
+    const int r = ok ? row / a.group : 0;
+    const uint16_t* src = a.q + static_cast<size_t>(rq.q0 + r) * a.q_stride +
+                          static_cast<size_t>(head * a.group + (row - r * a.group)) * HD + t * (HD / 4);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < HD / 32; ++w) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (ok) x = *reinterpret_cast<const uint4*>(src + 8 * w);
+      float f[8];
+      unpack8(x, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += f[i];
+      s.q[w][0][k] = __byte_perm(x.x, x.z, 0x5410);
+      s.q[w][0][RowState<HD, ROWS>::kR + k] = __byte_perm(x.y, x.w, 0x5410);
+      s.q[w][1][k] = __byte_perm(x.x, x.z, 0x7632);
+      s.q[w][1][RowState<HD, ROWS>::kR + k] = __byte_perm(x.y, x.w, 0x7632);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    s.qsum[k] = sum * a.scale_log2;
+    s.m[k] = -INFINITY;
+    s.l[k] = 0.f;
+    s.pb[k] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s.o[i][c] = 0.f;
+  s.unit = 0.f;
+}
+
+// One tile.  MASK: some of its keys are not seen by some row (limit[k]: keys of the tile that row k sees) or
+// lie in a page that was not loaded (page_ok: a bit for each).
+template <int HD, int ROWS, bool MASK>
+__device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, float scale_log2, const int* limit,
+                                         unsigned page_ok, int lane, RowState<HD, ROWS>& s) {
+  constexpr int kR = ROWS / 8;
+  const int g = lane >> 2, t = lane & 3;
+  const int sub_bytes = kv4_head_bytes(sub_shift, HD);
+  const int krow = (g >> 1) + 4 * (g & 1);  // column g of a score MMA is this key of its eight
+  float z[kTile / 8][2 * kR];
+  float top[kR];
+#pragma unroll
+  for (int k = 0; k < kR; ++k) top[k] = s.m[k];
+#pragma unroll
+  for (int i = 0; i < kTile / 8; ++i) {
+    const int j0 = 8 * i, sub = j0 >> sub_shift, at = j0 & ((1 << sub_shift) - 1);
+    const uint8_t* b = tile + sub * sub_bytes;
+    uint32_t w[HD / 32];
+    const uint8_t* src = b + (at + krow) * (HD / 2) + t * (HD / 8);
+    if constexpr (HD == 32) {
+      w[0] = *reinterpret_cast<const uint32_t*>(src);
+    } else if constexpr (HD == 64) {
+      const uint2 v = *reinterpret_cast<const uint2*>(src);
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(src);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+    float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+      const uint32_t x = w[u], y = x >> 8;
+      const uint32_t* q0 = s.q[u][0];
+      const uint32_t* q1 = s.q[u][1];
+      if constexpr (ROWS == 8) {
+        mma_16816(even, q0[0], 0u, q0[1], 0u, x & 0x000f000fu, y & 0x000f000fu);
+        mma_16816(odd, q1[0], 0u, q1[1], 0u, x & 0x00f000f0u, y & 0x00f000f0u);
+      } else {
+        mma_16816(even, q0[0], q0[1], q0[2], q0[3], x & 0x000f000fu, y & 0x000f000fu);
+        mma_16816(odd, q1[0], q1[1], q1[2], q1[3], x & 0x00f000f0u, y & 0x00f000f0u);
+      }
+    }
+    // this lane's two keys of the eight: t and 4 + t
+    const uint8_t* par = b + kv4_k_par(sub_shift, HD) + (at + t) * 4;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const __half2 h = *reinterpret_cast<const __half2*>(par + 16 * c);
+      const float2 f = __half22float2(h);
+      const float step = f.x * (scale_log2 * 16777216.f);
+#pragma unroll
+      for (int k = 0; k < kR; ++k) {
+        float v = fmaf(fmaf(odd[2 * k + c], 0.0625f, even[2 * k + c]), step, f.y * s.qsum[k]);
+        if constexpr (MASK) {
+          const int j = j0 + 4 * c + t;
+          if (j >= limit[k] || !(page_ok >> sub & 1u)) v = -INFINITY;
+        }
+        z[i][2 * k + c] = v;
+        top[k] = fmaxf(top[k], v);
+      }
+    }
+  }
+  // the greatest step among the tile's values sets the unit of the weights
+  uint32_t most = 0;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int j = lane + 32 * c, sub = j >> sub_shift, at = j & ((1 << sub_shift) - 1);
+    uint32_t h = *reinterpret_cast<const uint16_t*>(tile + sub * sub_bytes + kv4_v_par(sub_shift, HD) + at * 4);
+    if constexpr (MASK) {
+      if (j >= limit[kR] || !(page_ok >> sub & 1u)) h = 0;  // limit[kR]: keys that any row sees
+    }
+    if (h < 0x7c00u) most = max(most, h);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  // the power of two above the step: its fp32 exponent, plus one
+  const float step_unit =
+      __uint_as_float((__float_as_uint(h2f(static_cast<uint16_t>(most))) & 0x7f800000u) + 0x00800000u);
+  const float unit = most ? fmaxf(s.unit, step_unit) : s.unit;
+  const float per_unit = unit > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;  // 1 / unit
+  const float rescale = s.unit * per_unit;
+  s.unit = unit;
+  float fix[kR];
+  bool changed = rescale != 1.f;
+#pragma unroll
+  for (int k = 0; k < kR; ++k) {
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+    const float base = top[k] == -INFINITY ? 0.f : top[k];
+    const float keep = ex2(s.m[k] - base);
+    changed |= keep != 1.f;
+    s.m[k] = top[k];
+    s.l[k] *= keep;
+    s.pb[k] *= keep;
+    fix[k] = keep * rescale;
+    top[k] = base;
+  }
+  if (__any_sync(0xffffffffu, changed)) {
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      s.o[i][0] *= fix[0];
+      s.o[i][1] *= fix[0];
+      s.o[i][2] *= fix[kR - 1];
+      s.o[i][3] *= fix[kR - 1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kTile / 16; ++i) {
+    const int j0 = 16 * i, sub = j0 >> sub_shift, at = j0 & ((1 << sub_shift) - 1);
+    const uint8_t* b = tile + sub * sub_bytes;
+    const uint8_t* par = b + kv4_v_par(sub_shift, HD) + (at + t) * 4;
+    uint32_t hi[kR][2], lo[kR][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {  // keys 8 c + t and 8 c + 4 + t
+      float wt[kR][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const __half2 h = *reinterpret_cast<const __half2*>(par + 32 * c + 16 * e);
+        const float2 f = __half22float2(h);
+        const float step = f.x * per_unit;
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          const float v = z[2 * i + c][2 * k + e];
+          float p = ex2(v - top[k]);
+          float low = f.y, st = step;
+          if constexpr (MASK) {
+            const int j = j0 + 8 * c + 4 * e + t;
+            if (j >= limit[k] || !(page_ok >> sub & 1u)) p = low = st = 0.f;
+          }
+          s.l[k] += p;
+          s.pb[k] = fmaf(p, low, s.pb[k]);
+          wt[k][e] = p * st;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kR; ++k) split2(wt[k][0], wt[k][1], &hi[k][c], &lo[k][c]);
+    }
+    const auto add = [&](int n, uint32_t b0, uint32_t b1) {
+      if constexpr (ROWS == 8) {
+        mma_16816(s.o[n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
+      } else {
+        mma_16816(s.o[n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
+        mma_16816(s.o[n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
+      }
+    };
+    const auto four = [&](int n, uint32_t x, uint32_t y) {  // four nibbles of two pairs of tokens
+      add(n, x & 0x000f000fu, y & 0x000f000fu);
+      add(n + 1, x & 0x00f000f0u, y & 0x00f000f0u);
+      x >>= 8, y >>= 8;
+      add(n + 2, x & 0x000f000fu, y & 0x000f000fu);
+      add(n + 3, x & 0x00f000f0u, y & 0x00f000f0u);
+    };
+    const uint8_t* src = b + kv4_v_codes(sub_shift, HD) + (at + t) * (HD / 2);
+    if constexpr (HD == 32) {
+      uint32_t x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const uint32_t*>(src + 4 * c * (HD / 2) + (g >> 1) * 4);
+      const uint32_t pick = (g & 1) ? 0x7632u : 0x5410u;
+      four(0, __byte_perm(x[0], x[1], pick), __byte_perm(x[2], x[3], pick));
+    } else if constexpr (HD == 64) {
+      uint32_t x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const uint32_t*>(src + 4 * c * (HD / 2) + g * 4);
+      four(0, __byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410));
+      four(4, __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
+    } else {
+      uint2 x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const uint2*>(src + 4 * c * (HD / 2) + g * 8);
+      four(0, __byte_perm(x[0].x, x[1].x, 0x5410), __byte_perm(x[2].x, x[3].x, 0x5410));
+      four(4, __byte_perm(x[0].x, x[1].x, 0x7632), __byte_perm(x[2].x, x[3].x, 0x7632));
+      four(8, __byte_perm(x[0].y, x[1].y, 0x5410), __byte_perm(x[2].y, x[3].y, 0x5410));
+      four(12, __byte_perm(x[0].y, x[1].y, 0x7632), __byte_perm(x[2].y, x[3].y, 0x7632));
+    }
+  }
+}
+
+// Where query row `row` of a request's kv head goes.
+__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, const Request& rq, int head, int row, int hd) {
+  const int r = row / a.group;
+  return a.out + static_cast<size_t>(rq.q0 + r) * a.out_stride +
+         static_cast<size_t>(head * a.group + row - r * a.group) * hd;
+}
+
+// Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.
+template <int HD, int ROWS>
+__device__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int block, int first, int last, int lane) {
+  constexpr int kD = HD / 32;
+  const int rows = min(ROWS, rq.n * a.group - block * ROWS);
+  const size_t stride = static_cast<size_t>(2) * ROWS * kRecord<HD>;  // from a warp's records to the next's
+  for (int row = 0; row < rows; ++row) {
+    // the first warp's piece is its last one (second record), the others' their first
+    const float* r0 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + ROWS + row) * kRecord<HD>;
+    const float* r1 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + row) * kRecord<HD>;
+    const int n = last - first + 1;
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? r1 + i * stride : r0)[0]);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[kD];
+#pragma unroll
+    for (int d = 0; d < kD; ++d) acc[d] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* r = i ? r1 + i * stride : r0;
+      const float w = ex2(r[0] - base);
+      sum = fmaf(w, r[1], sum);
+#pragma unroll
+      for (int d = 0; d < kD; ++d) acc[d] = fmaf(w, r[4 + lane + 32 * d], acc[d]);
+    }
+    uint16_t* o = out_row(a, rq, head, block * ROWS + row, HD);
+#pragma unroll
+    for (int d = 0; d < kD; ++d) o[lane + 32 * d] = f2h(sum == 0.f ? 0.f : acc[d] / sum);
+  }
+}
+
+template <int HD, int ROWS>
+__global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_split_kernel(const AttnArgs a) {
+  constexpr int kR = ROWS / 8;
+  constexpr int kS = kStages<HD>;
+  constexpr int kThreads = kSplitWarps * 32;
+  extern __shared__ __align__(128) uint8_t split_smem[];
+  __shared__ uint64_t bars[kSplitWarps][kS];
+  __shared__ long long s_before[kThreads + 1];
+  __shared__ int s_most;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = split_smem + warp * kS * kTileBytes<HD>;
+
+  // the line of units: each thread sums a run of requests
+  const int per = (a.n_seq + kThreads - 1) / kThreads;
+  if (tid == 0) s_most = 0;
+  if (lane < kS) mbar_init(&bars[warp][lane], 1);
+  fence_barrier_init();
+  __syncthreads();
+  {
+    long long mine = 0;
+    int most = 0;
+    for (int s = tid * per; s < min((tid + 1) * per, a.n_seq); ++s)
+      mine += a.kv_heads * head_units<ROWS>(a, request_of(a, s), &most);
+    atomicMax(&s_most, most);
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    s_before[tid + 1] = inc;
+    __syncthreads();
+    long long add = 0;
+    for (int w = 0; w < warp; ++w) add += s_before[32 * (w + 1)];
+    __syncthreads();
+    s_before[tid + 1] = inc + add;
+    if (tid == 0) s_before[0] = 0;
+    __syncthreads();
+  }
+  const long long total = s_before[kThreads];
+  const int warps = static_cast<int>(gridDim.x) * kSplitWarps;
+  const int me = static_cast<int>(blockIdx.x) * kSplitWarps + warp;
+  // a run: an equal share, and no less than lets kMaxPieces warps cover the longest item
+  const long long share = max((total + warps - 1) / warps, static_cast<long long>((s_most + kMaxPieces - 1) / kMaxPieces));
+  const long long u0 = me * share, u1 = min(total, u0 + share);
+  if (u0 >= u1) return;
+
+  // the request that holds unit u0, then the head, block and tile
+  Cursor<ROWS> at;
+  long long item_start;  // unit of the current item's tile 0
+  {
+    int lo = 0, hi = kThreads;  // the last run of requests that starts at or before u0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_before[mid] <= u0) {
+        lo = mid;
+      } else {
+        hi = mid;
+      }
+    }
+    long long left = u0 - s_before[lo];
+    int s = lo * per, most = 0;
+    long long u = 1;
+    for (;; s += 32) {  // a lane to a request of the run
+      const long long mine = s + lane < a.n_seq ? head_units<ROWS>(a, request_of(a, s + lane), &most) : 0;
+      long long inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned here = __ballot_sync(0xffffffffu, left < inc * a.kv_heads);
+      if (here) {
+        const int i = __ffs(static_cast<int>(here)) - 1;
+        s += i;
+        u = __shfl_sync(0xffffffffu, mine, i);
+        left -= __shfl_sync(0xffffffffu, inc - mine, i) * a.kv_heads;
+        break;
+      }
+      left -= __shfl_sync(0xffffffffu, inc, 31) * a.kv_heads;
+      if (s + 32 >= a.n_seq) return;  // not reached: u0 lies on the line
+    }
+    const int head = static_cast<int>(left / u);
+    left -= head * u;
+    at.enter(a, s, head, 0);
+    while (left >= at.tiles && at.block + 1 < at.blocks) {
+      left -= at.tiles;
+      at.tiles = tiles_of<ROWS>(a, at.req, ++at.block);
+    }
+    at.tile = static_cast<int>(left);
+    item_start = u0 - left;
+  }
+
+  const int sub_shift = min(a.shift, 6), subs = kTile >> sub_shift;  // pages of a tile, or parts of one
+  // The copies run kS tiles ahead of the sums; the page of the next copy is
+  // read one tile earlier still, so that nothing waits for it.
+  Cursor<ROWS> ahead = at;
+  long long to_load = u1 - u0;
+  int page = -1;
+  const auto fetch_page = [&]() {
+    page = -1;
+    if (to_load > 0 && lane < subs) {
+      const int last = min((ahead.block + 1) * ROWS, ahead.req.n * a.group) - 1;
+      const int j = ahead.tile * kTile + (lane << sub_shift);
+      if (j < limit_of(a, ahead.req, last / a.group))
+        page = a.table[static_cast<size_t>(ahead.seq) * a.max_blocks + (j >> a.shift)];
+    }
+  };
+  unsigned ok_bits[kS];
+  const auto issue = [&](int stage, uint64_t* bar) -> unsigned {
+    const bool ok = page >= 0 && page < a.n_pages;
+    const unsigned mask = __ballot_sync(0xffffffffu, ok);
+    const int bytes = kv4_head_bytes(sub_shift, HD);
+    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(mask) * bytes);
+    __syncwarp();
+    if (ok) {
+      const uint8_t* src = a.pages + static_cast<size_t>(page) * a.page_bytes +
+                           static_cast<size_t>(ahead.head) * kv4_head_bytes(a.shift, HD);
+      uint8_t* dst = ring + stage * kTileBytes<HD> + lane * bytes;
+      if (a.shift <= 6) {
+        bulk_load(dst, src, bytes, bar);
+      } else {  // half of a page of 128: its four parts
+        const int half = ahead.tile & 1;
+        const int codes = kv4_v_codes(6, HD);
+        bulk_load(dst, src + half * codes, codes, bar);
+        bulk_load(dst + codes, src + kv4_v_codes(7, HD) + half * codes, codes, bar);
+        bulk_load(dst + kv4_k_par(6, HD), src + kv4_k_par(7, HD) + half * 256, 256, bar);
+        bulk_load(dst + kv4_v_par(6, HD), src + kv4_v_par(7, HD) + half * 256, 256, bar);
+      }
+    }
+    --to_load;
+    if (to_load > 0) {
+      if (++ahead.tile == ahead.tiles) ahead.next_item(a);
+      fetch_page();
+    }
+    return mask;
+  };
+  fetch_page();
+#pragma unroll
+  for (int st = 0; st < kS; ++st) ok_bits[st] = to_load > 0 ? issue(st, &bars[warp][st]) : 0u;
+
+  RowState<HD, ROWS> s;
+  int stage = 0;
+  uint32_t parity = 0;
+  long long u = u0;
+  bool alive = true;
+  while (u < u1) {
+    const int t1 = static_cast<int>(min(static_cast<long long>(at.tiles), at.tile + (u1 - u)));
+    load_rows<HD, ROWS>(a, at.req, at.head, at.block, lane, s);
+    int limit[kR + 1];
+    int least = 0x7fffffff;
+    {
+      const int rows = at.req.n * a.group, row0 = at.block * ROWS;
+      least = limit_of(a, at.req, row0 / a.group);
+#pragma unroll
+      for (int k = 0; k < kR; ++k)
+        limit[k] = limit_of(a, at.req, min(row0 + 8 * k + (lane >> 2), rows - 1) / a.group);
+      limit[kR] = limit_of(a, at.req, (min(row0 + ROWS, rows) - 1) / a.group);
+    }
+    for (int tile = at.tile; tile < t1; ++tile, ++u) {
+      if (alive) alive = mbar_wait(&bars[warp][stage], parity, a.status);
+      if (!__all_sync(0xffffffffu, alive)) {
+        alive = false;
+        break;
+      }
+      unsigned ok = 0;
+#pragma unroll
+      for (int st = 0; st < kS; ++st) ok = st == stage ? ok_bits[st] : ok;
+      const uint8_t* buf = ring + stage * kTileBytes<HD>;
+      const int j0 = tile * kTile;
+      if (j0 + kTile <= least && ok == (1u << subs) - 1u) {
+        add_tile<HD, ROWS, false>(buf, sub_shift, a.scale_log2, nullptr, 0, lane, s);
+      } else {
+        int rel[kR + 1];
+#pragma unroll
+        for (int k = 0; k <= kR; ++k) rel[k] = limit[k] - j0;
+        add_tile<HD, ROWS, true>(buf, sub_shift, a.scale_log2, rel, ok, lane, s);
+      }
+      __syncwarp();  // every lane has read the tile
+      if (to_load > 0) {
+        const unsigned got = issue(stage, &bars[warp][stage]);
+#pragma unroll
+        for (int st = 0; st < kS; ++st) ok_bits[st] = st == stage ? got : ok_bits[st];
+      }
+      if (++stage == kS) {
+        stage = 0;
+        parity ^= 1u;
+      }
+    }
+    if (!alive) break;
+    // the item's rows so far: sums over the lanes of a row, and the codes' unit
+    const bool whole = at.tile == 0 && t1 == at.tiles;
+    const int first = static_cast<int>(item_start / share), last = static_cast<int>((item_start + at.tiles - 1) / share);
+    const float up = s.unit * 16777216.f;
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      float l = s.l[k], pb = s.pb[k];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      pb += __shfl_xor_sync(0xffffffffu, pb, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      pb += __shfl_xor_sync(0xffffffffu, pb, 2);
+      const int in_block = 8 * k + (lane >> 2), row = at.block * ROWS + in_block;
+      if (row < at.req.n * a.group) {
+        float v[HD / 4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float sum = ROWS == 8 ? s.o[i][c] + s.o[i][2 + c] : s.o[i][2 * k + c];
+            v[c * (HD / 8) + i] = fmaf(sum, (i & 1) ? up * 0.0625f : up, pb);
+          }
+        if (whole) {
+          uint16_t* o = out_row(a, at.req, at.head, row, HD) + (lane & 3) * (HD / 4);
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              h[j] = l == 0.f ? 0u : f2h2(v[8 * i + 2 * j] * inv, v[8 * i + 2 * j + 1] * inv);
+            *reinterpret_cast<uint4*>(o + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        } else {
+          float* r = a.parts + (static_cast<size_t>(me) * 2 * ROWS + (me == first ? ROWS : 0) + in_block) * kRecord<HD>;
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(r) = make_float2(s.m[k], l);
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i)
+            *reinterpret_cast<float4*>(r + 4 + (lane & 3) * (HD / 4) + 4 * i) =
+                make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncwarp();
+      int n = 0;
+      if (lane == 0) n = atomicAdd(a.tickets + first, 1);
+      n = __shfl_sync(0xffffffffu, n, 0);
+      if (n == last - first) {
+        __threadfence();
+        join_pieces<HD, ROWS>(a, at.req, at.head, at.block, first, last, lane);
+        if (lane == 0) a.tickets[first] = 0;
+      }
+    }
+    item_start += at.tiles;
+    if (u < u1) at.next_item(a);
+  }
+  if (!alive) {  // a copy never came: leave once those in flight have landed, as far as waits go
+    for (int st = 0; st < kS; ++st) mbar_wait(&bars[warp][st], parity ^ (st < stage ? 1u : 0u), a.status);
+  }
+}
+
+template <int HD, int ROWS>
+int launch_split(const AttnArgs& a, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(kSplitWarps) * kStages<HD> * kTileBytes<HD>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kv4_attn_split_kernel<HD, ROWS>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(smem)),
+                            "cudaFuncSetAttribute(kv4_attn_split)"))
+      return rc;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  kv4_attn_split_kernel<HD, ROWS>
+      <<<static_cast<unsigned>(sm_count() * kCtasPerSm<HD>), kSplitWarps * 32, smem, st>>>(a);
+  return check_launch("kv4_attn_split_kernel");
+}
+
+// Tickets (zero between calls), then the records.
+size_t split_warps(size_t hd) {
+  return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128> : hd == 64 ? kCtasPerSm<64> : kCtasPerSm<32>);
+}
+size_t tickets_bytes(size_t hd) { return (split_warps(hd) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
 
 }  // namespace
 }  // namespace gsvk
@@ -117,7 +717,7 @@ size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads,
       heads == 0 || heads > 65536 || n_tokens > 0x7fffffff ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return 0;
-  return 256;
+  return tickets_bytes(head_dim) + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float);
 }
 
 int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
@@ -165,13 +765,15 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   a.prefix = g->prefix;
   a.table = g->block_table;
   a.scale_log2 = g->scale * 1.4426950408889634f;
-  const size_t items = g->n_tokens * g->heads;
-  const unsigned blocks = ceil_div(items, kSimpleWarps);
+  a.tickets = static_cast<int*>(g->workspace);
+  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + tickets_bytes(hd));
+  a.status = device_status();
   cudaStream_t st = as_cuda(stream);
-  if (hd == 32) kv4_attn_rows_kernel<32><<<blocks, kSimpleWarps * 32, 0, st>>>(a);
-  if (hd == 64) kv4_attn_rows_kernel<64><<<blocks, kSimpleWarps * 32, 0, st>>>(a);
-  if (hd == 128) kv4_attn_rows_kernel<128><<<blocks, kSimpleWarps * 32, 0, st>>>(a);
-  return check_launch("kv4_attn_rows_kernel");
+  // up to 8 rows to a kv head leave half of an MMA's rows to the weights' second parts
+  if (g->max_q * a.group <= 8) {
+    return hd == 32 ? launch_split<32, 8>(a, st) : hd == 64 ? launch_split<64, 8>(a, st) : launch_split<128, 8>(a, st);
+  }
+  return hd == 32 ? launch_split<32, 16>(a, st) : hd == 64 ? launch_split<64, 16>(a, st) : launch_split<128, 16>(a, st);
 }
 
 }  // extern "C"
