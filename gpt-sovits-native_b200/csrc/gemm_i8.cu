@@ -55,6 +55,308 @@ __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bia
   return apply_act(fmaf(static_cast<float>(acc), sa * sb, bias), e.act, e.slope);
 }
 
+// ------------------------------------------------------------- tensor cores
+// One persistent CTA per SM over 128 x BN output tiles.  Warp 0 loads K blocks
+// of 128 bytes of A and B by TMA into 128-byte swizzled stages, warp 1 issues
+// tcgen05.mma.kind::i8 (M 128, N BN, K 32; exact 32-bit sums in TMEM, two
+// accumulators of BN columns), and the epilogue warps turn one accumulator
+// into outputs while the next one fills.  TMA fills what lies past M, N and K
+// with zeros, so no size is special.
+//
+// Epilogue: a lane owns a row, 32 columns at a time.  Column scales and biases
+// reach it as broadcasts from a small shared-memory table per warp; results
+// go to a swizzled 32 x 32 tile, which leaves by a TMA store, or, where the
+// output's columns or stride are not whole 16 bytes, row by row.
+constexpr int kI8BM = 128;
+constexpr int kI8BK = 128;  // bytes of K per stage
+constexpr int kI8MaxStages = 8;
+
+template <int BN>
+constexpr int kI8EpiWarps = BN >= 128 ? 8 : 4;  // two column halves from 128 columns on
+template <int BN>
+constexpr int kI8Threads = 64 + 32 * kI8EpiWarps<BN>;
+
+struct I8Problem {
+  int M, N, K, m_tiles, n_tiles, stages;
+  int tma32, tma16;  // outputs that leave by TMA
+};
+
+// tcgen05 instruction descriptor of kind::i8: signed 8-bit A and B, K-major, 32-bit integer D.
+__host__ __device__ constexpr uint32_t idesc_i8(uint32_t M, uint32_t N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+constexpr int kI8Tile32 = 32 * 128, kI8Tile16 = 32 * 64;  // bytes of a staged 32 x 32 tile
+// 16-byte unit j of row r of a staged tile, in the swizzle of its TMA store.
+__device__ __forceinline__ uint8_t* unit32(uint8_t* tile, int r, int j) {
+  return tile + r * 128 + ((j ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ uint8_t* unit16(uint8_t* tile, int r, int j) {
+  return tile + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kI8Threads<BN>, 1)
+    gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tm32, const __grid_constant__ CUtensorMap tm16,
+                   const I8Problem prob, const I8Epilogue epi, uint32_t* status) {
+  constexpr uint32_t kABytes = kI8BM * kI8BK, kBBytes = BN * kI8BK;
+  constexpr uint32_t kTmemCols = 2 * BN;
+  constexpr int kEpi = kI8EpiWarps<BN>;
+  const I8Problem p = prob;
+  const I8Epilogue e = epi;
+  extern __shared__ uint8_t i8_raw[];
+  uint8_t* smem = align_smem<1024>(i8_raw);
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + p.stages * kABytes;
+  uint8_t* sOut = sB + p.stages * kBBytes;  // per epilogue warp: two fp32 and two fp16 tiles, as far as needed
+  const int out_bytes = 2 * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
+  __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float2 s_col[kEpi][32];  // column scale and bias of a warp's chunk
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int kbn = (p.K + kI8BK - 1) / kI8BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], kEpi);
+    }
+    fence_barrier_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    if (p.tma32) prefetch_tmap(&tm32);
+    if (p.tma16) prefetch_tmap(&tm16);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  griddep_wait();  // operands may come from the previous kernel (the row quantiser)
+  griddep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
+        for (int kb = 0; kb < kbn; ++kb, ++it) {
+          const int s = it % p.stages;
+          if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / p.stages) & 1u) ^ 1u, status)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
+          tma_load_2d(sA + s * kABytes, &tmA, &full[s], kb * kI8BK, mt * kI8BM);
+          tma_load_2d(sB + s * kBBytes, &tmB, &full[s], kb * kI8BK, nt * BN);
+        }
+      }
+      if (!ok)  // a wait ran out: leave once the loads in flight have landed
+        for (int i = max(0, it - p.stages); i < it; ++i)
+          mbar_wait(&full[i % p.stages], static_cast<uint32_t>(i / p.stages) & 1u, status);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(kI8BM, BN);
+      int it = 0, tl = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++tl) {
+        const int acc = tl & 1;
+        if (!mbar_wait(&tempty[acc], (static_cast<uint32_t>(tl >> 1) & 1u) ^ 1u, status)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < kbn; ++kb, ++it) {
+          const int s = it % p.stages;
+          if (!mbar_wait(&full[s], static_cast<uint32_t>(it / p.stages) & 1u, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(sA + s * kABytes), b = smem_u32(sB + s * kBBytes);
+#pragma unroll
+          for (int j = 0; j < kI8BK / 32; ++j)
+            tc_mma_i8(tmem + acc * BN, smem_desc(a + 32u * j, 1024, 2), smem_desc(b + 32u * j, 1024, 2), idesc,
+                      (kb | j) ? 1u : 0u);
+          tc_commit(&empty[s]);
+        }
+        if (ok) tc_commit(&tfull[acc]);
+      }
+    }
+  } else {
+    const int w = warp - 2, quarter = warp & 3;  // TMEM lanes 32 quarter .. + 31
+    constexpr int kSpan = kEpi == 8 ? BN / 2 : BN;
+    const int cbeg = kEpi == 8 ? (w >> 2) * kSpan : 0;
+    uint8_t* out32 = sOut + w * out_bytes;
+    uint8_t* out16 = out32 + (e.c32 ? 2 * kI8Tile32 : 0);
+    int turn = 0, tl = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++tl) {
+      const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
+      const int acc = tl & 1;
+      const int row0 = mt * kI8BM + quarter * 32, row = row0 + lane;
+      const float sa = row < p.M ? e.a_scale[row] : 0.f;
+      const auto column = [&](int c) {
+        const int n = nt * BN + c + lane;
+        return n < p.N ? make_float2(__ldg(e.b_scale + n), e.bias ? __ldg(e.bias + n) : 0.f) : make_float2(0.f, 0.f);
+      };
+      float2 col = column(cbeg);
+      if (!mbar_wait(&tfull[acc], static_cast<uint32_t>(tl >> 1) & 1u, status)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = cbeg; c0 < cbeg + kSpan; c0 += 32) {
+        const int n0 = nt * BN + c0;
+        if (n0 >= p.N) break;
+        s_col[w][lane] = col;
+        if (c0 + 32 < cbeg + kSpan) col = column(c0 + 32);
+        uint32_t r[32];
+        const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + c0;
+        tmem_ld16(from, r);
+        tmem_ld16(from + 16, r + 16);
+        // the stores that read this turn's tiles are done with them
+        if (lane == 0 && (p.tma32 || p.tma16)) bulk_wait_read<1>();
+        tmem_ld_wait();
+        __syncwarp();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float4 c = *reinterpret_cast<const float4*>(&s_col[w][j]);
+          v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])), sa * c.x, c.y);
+          v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])), sa * c.z, c.w);
+        }
+        act_array<32>(v, e.act, e.slope);
+        if (e.residual && row < p.M) {
+          const float* res = e.residual + row * e.ld_res + n0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (n0 + j < p.N) v[j] += res[j];
+        }
+        uint8_t* t32 = out32 + (turn & 1) * kI8Tile32;
+        uint8_t* t16 = out16 + (turn & 1) * kI8Tile16;
+        if (e.c32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(unit32(t32, lane, j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        if (e.c16) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(unit16(t16, lane, j)) =
+                make_uint4(f2h2(v[8 * j], v[8 * j + 1]), f2h2(v[8 * j + 2], v[8 * j + 3]),
+                           f2h2(v[8 * j + 4], v[8 * j + 5]), f2h2(v[8 * j + 6], v[8 * j + 7]));
+        }
+        if (p.tma32 || p.tma16) fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0 && row0 < p.M) {
+          if (p.tma32) tma_store_2d(&tm32, t32, n0, row0);
+          if (p.tma16) tma_store_2d(&tm16, t16, n0, row0);
+        }
+        if (lane == 0 && (p.tma32 || p.tma16)) bulk_commit();
+        if ((e.c32 && !p.tma32) || (e.c16 && !p.tma16)) {  // row by row, a lane to a column
+          const int rows = min(32, p.M - row0);
+          if (n0 + lane < p.N) {
+#pragma unroll 8
+            for (int i = 0; i < rows; ++i) {
+              if (e.c32 && !p.tma32)
+                e.c32[(row0 + i) * e.ld_c32 + n0 + lane] =
+                    *reinterpret_cast<const float*>(unit32(t32, i, lane >> 2) + 4 * (lane & 3));
+              if (e.c16 && !p.tma16)
+                e.c16[(row0 + i) * e.ld_c16 + n0 + lane] =
+                    *reinterpret_cast<const uint16_t*>(unit16(t16, i, lane >> 3) + 2 * (lane & 7));
+            }
+          }
+          __syncwarp();
+        }
+        ++turn;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+    }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+int i8_map(CUtensorMap* m, const int8_t* base, size_t rows, size_t K, size_t ld, int box_rows) {
+  const uint64_t dims[2] = {K, rows};
+  const uint64_t strides[1] = {ld};
+  const uint32_t box[2] = {kI8BK, static_cast<uint32_t>(box_rows)};
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN>
+int launch_i8(const gsvk_gemm_i8_args* g, size_t lda, size_t ldb, const I8Epilogue& e, cudaStream_t st) {
+  I8Problem p{};
+  p.M = static_cast<int>(g->M);
+  p.N = static_cast<int>(g->N);
+  p.K = static_cast<int>(g->K);
+  p.m_tiles = (p.M + kI8BM - 1) / kI8BM;
+  p.n_tiles = (p.N + BN - 1) / BN;
+  CUtensorMap ta, tb, t32{}, t16{};
+  int rc = i8_map(&ta, g->a, g->M, g->K, lda, kI8BM);
+  if (!rc) rc = i8_map(&tb, g->b, g->N, g->K, ldb, BN);
+  // a TMA store writes whole 16 bytes of a row: the columns have to be, beside the stride
+  const uint64_t odims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)};
+  const uint32_t box[2] = {32, 32};
+  if (!rc && e.c32 && aligned16(e.c32) && e.ld_c32 % 4 == 0 && p.N % 4 == 0) {
+    const uint64_t str[1] = {static_cast<uint64_t>(e.ld_c32) * 4};
+    rc = encode_tiled(&t32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, e.c32, odims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    p.tma32 = 1;
+  }
+  if (!rc && e.c16 && aligned16(e.c16) && e.ld_c16 % 8 == 0 && p.N % 8 == 0) {
+    const uint64_t str[1] = {static_cast<uint64_t>(e.ld_c16) * 2};
+    rc = encode_tiled(&t16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, e.c16, odims, str, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    p.tma16 = 1;
+  }
+  if (rc) return rc;
+  constexpr size_t kLimit = 227 * 1024 - 4096;  // barriers and column tables are static
+  const size_t staging = static_cast<size_t>(kI8EpiWarps<BN>) * 2 * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
+  const size_t stage = (kI8BM + BN) * kI8BK;
+  const int kbn = (p.K + kI8BK - 1) / kI8BK;
+  p.stages = static_cast<int>(std::min<size_t>(kI8MaxStages, (kLimit - 1024 - staging) / stage));
+  // no more stages than this CTA has K blocks to load
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const long long rounds = (tiles + sm_count() - 1) / sm_count();
+  p.stages = static_cast<int>(std::max<long long>(1, std::min<long long>(p.stages, rounds * kbn)));
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    rc = check_cuda(cudaFuncSetAttribute(gemm_i8_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kLimit)),
+                    "cudaFuncSetAttribute(gemm_i8)");
+    if (rc) return rc;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  const size_t smem = 1024 + p.stages * stage + staging;
+  return launch_pdl(gemm_i8_kernel<BN>, dim3(static_cast<unsigned>(std::min<long long>(tiles, sm_count()))),
+                    dim3(kI8Threads<BN>), smem, st, "gemm_i8_kernel", ta, tb, t32, t16, p, e, device_status());
+}
+
 // Operands in any layout: one thread to an output, bytes in order.
 __global__ void __launch_bounds__(256)
     gemm_i8_simt_kernel(const int8_t* __restrict__ a, long long lda, const int8_t* __restrict__ b,
@@ -110,9 +412,20 @@ int gsvk_gemm_i8(const gsvk_gemm_i8_args* g, gsvk_stream_t stream) {
   if (g->act < GSVK_ACT_NONE || g->act > GSVK_ACT_TANH) return fail(GSVK_ERR_INVALID, "gemm_i8: bad act");
   I8Epilogue e{g->a_scale, g->b_scale, g->bias, g->residual, g->c, g->c_f16,
                (long long)ldr, (long long)ldc, (long long)ldh, g->act, g->slope};
+  cudaStream_t st = as_cuda(stream);
+  if (gsvk_available() && aligned16(g->a) && aligned16(g->b) && (lda % 16 == 0 || g->M == 1) && (ldb % 16 == 0 || g->N == 1)) {
+    // one row: any stride will do
+    const size_t sa = g->M == 1 ? (g->K + 15) / 16 * 16 : lda, sb = g->N == 1 ? (g->K + 15) / 16 * 16 : ldb;
+    // the widest tile whose tiles still fill the GPU: each A byte then feeds the most columns
+    const size_t m_tiles = (g->M + kI8BM - 1) / kI8BM, sms = static_cast<size_t>(sm_count());
+    if (m_tiles * ((g->N + 255) / 256) >= sms) return launch_i8<256>(g, sa, sb, e, st);
+    if (m_tiles * ((g->N + 127) / 128) >= sms) return launch_i8<128>(g, sa, sb, e, st);
+    if (m_tiles * ((g->N + 63) / 64) >= sms) return launch_i8<64>(g, sa, sb, e, st);
+    return launch_i8<32>(g, sa, sb, e, st);
+  }
   const size_t outs = g->M * g->N;
   if (ceil_div(outs, 256) > 0x7fffffff) return fail(GSVK_ERR_UNSUPPORTED, "gemm_i8: too big");
-  gemm_i8_simt_kernel<<<ceil_div(outs, 256), 256, 0, as_cuda(stream)>>>(
+  gemm_i8_simt_kernel<<<ceil_div(outs, 256), 256, 0, st>>>(
       g->a, (long long)lda, g->b, (long long)ldb, (long long)g->M, (int)g->N, (int)g->K, e);
   return check_launch("gemm_i8_simt_kernel");
 }
