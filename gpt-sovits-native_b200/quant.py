@@ -19,7 +19,7 @@ from __future__ import annotations
 import ctypes
 from ctypes import byref, c_float, c_int, c_size_t, c_void_p
 
-from . import ACT_NONE, _stream, check, lib
+from . import ACT_NONE, check, lib
 
 _vp, _sz = c_void_p, c_size_t
 
@@ -51,25 +51,47 @@ class GemmI8Args(ctypes.Structure):
                 ("ldc_f16", _sz), ("act", c_int), ("slope", c_float)]
 
 
-def _tensor(t, dtype, what, dim=None):
-    """A CUDA tensor of one type whose rows are contiguous; its address."""
+_raw_stream = None
+
+
+def _stream_for(stream, t):
+    """Handle of `stream`, or of the current stream of t's device.  At a decode
+    step's sizes a call takes a few microseconds, which making a Stream object
+    (torch.cuda.current_stream) would double: torch's raw handle is read instead
+    where it is to be had."""
+    global _raw_stream
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:
+        import torch
+
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(t.get_device())
+
+
+def _tensor(t, dtype, dim, what):
+    """Address of a CUDA tensor of one type and rank whose rows are contiguous."""
+    if t.dtype is dtype and t.is_cuda and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] < 2):
+        return t.data_ptr()
     if not t.is_cuda:
         raise ValueError(f"{what}: gsvk takes CUDA tensors")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{what}: {dtype} expected, got {t.dtype}")
-    if dim is not None and t.dim() != dim:
+    if t.dim() != dim:
         raise ValueError(f"{what}: {dim} dimensions expected, got {t.dim()}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: gsvk takes tensors with unit inner stride")
-    return t.data_ptr()
+    raise ValueError(f"{what}: gsvk takes tensors with unit inner stride")
 
 
 def _vector(t, dtype, n, what):
-    """Address of a contiguous vector of at least n values."""
-    p = _tensor(t, dtype, what)
-    if t.numel() < n or not t.is_contiguous():
-        raise ValueError(f"{what}: {n} contiguous values expected")
-    return p
+    """Address of at least n contiguous values."""
+    if t.dtype is dtype and t.is_cuda and t.is_contiguous() and t.numel() >= n:
+        return t.data_ptr()
+    if not t.is_cuda:
+        raise ValueError(f"{what}: gsvk takes CUDA tensors")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {dtype} expected, got {t.dtype}")
+    raise ValueError(f"{what}: {n} contiguous values expected")
 
 
 def _row_stride(t):
@@ -79,19 +101,18 @@ def _row_stride(t):
 
 def _rows(t, dtype, heads, head_dim, what):
     """Address and row stride of [tokens, heads, head_dim] rows whose heads lie side by side."""
-    p = _tensor(t, dtype, what, 3)
-    if t.shape[1] != heads or t.shape[2] != head_dim:
+    p = _tensor(t, dtype, 3, what)
+    n, h, d = t.shape
+    if h != heads or d != head_dim:
         raise ValueError(f"{what}: [tokens, {heads}, {head_dim}] expected, got {tuple(t.shape)}")
-    if heads > 1 and t.stride(1) != head_dim:
+    row, head, _ = t.stride()
+    if heads > 1 and head != head_dim:
         raise ValueError(f"{what}: the heads of a row lie side by side")
-    return p, t.stride(0) if t.shape[0] > 1 else heads * head_dim
+    return p, row if n > 1 else heads * head_dim
 
 
-def _new(shape, dtype, device, stream):
+def _kept(t, stream):
     """An output of this call, kept by the allocator until `stream` is done with it."""
-    import torch
-
-    t = torch.empty(shape, dtype=dtype, device=device)
     if stream is not None:
         t.record_stream(stream)
     return t
@@ -111,6 +132,7 @@ class KVPlan:
         i32 = dict(dtype=torch.int32, device=device)
         self.n_seq, self.max_blocks, self.n_pages = int(n_seq), int(max_blocks), int(n_pages)
         self.page_size, self.max_tokens = int(page_size), int(max_tokens)
+        self._table_shape = (self.n_seq, self.max_blocks)
         self.q_start = torch.zeros(n_seq + 1, **i32)
         self.kv_len = torch.zeros(n_seq, **i32)
         self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
@@ -127,8 +149,8 @@ class KVPlan:
         import torch
 
         i32 = torch.int32
-        if tuple(block_table.shape) != (self.n_seq, self.max_blocks):
-            raise ValueError(f"block_table: {(self.n_seq, self.max_blocks)} expected, got "
+        if block_table.shape != self._table_shape:
+            raise ValueError(f"block_table: {self._table_shape} expected, got "
                              f"{tuple(block_table.shape)}")
         return (_vector(length, i32, self.n_seq, "lengths"),
                 _vector(block_table, i32, 0, "block_table"),
@@ -150,7 +172,7 @@ class KVPlan:
         a.new_len = _vector(new_len, torch.int32, self.n_seq, "new_len")
         a.kv_len = a.ctx_len if in_place else self.kv_len.data_ptr()
         a.free_left = a.free_count if in_place else self.free_left.data_ptr()
-        check(lib().gsvk_kv_plan(byref(a), _stream(stream)))
+        check(lib().gsvk_kv_plan(byref(a), _stream_for(stream, block_table)))
         return self
 
     def release(self, done, length, block_table, free_pages, free_count, stream=None):
@@ -160,7 +182,7 @@ class KVPlan:
         ln, table, free, count = self._state(length, block_table, free_pages, free_count)
         check(lib().gsvk_kv_release(self.n_seq, self.max_blocks, self.n_pages, self.page_size,
                                     _vector(done, torch.int32, self.n_seq, "done"), ln, table, free,
-                                    count, _stream(stream)))
+                                    count, _stream_for(stream, block_table)))
 
 
 # ------------------------------------------------------------- 4-bit KV cache
@@ -204,6 +226,7 @@ class KV4Cache:
         self.n_pages = pages.numel() // size
         self._cache = KV4CacheArgs(p, self.n_pages, self.page_size, self.kv_heads, self.head_dim)
         self._attn = KV4AttentionArgs(cache=self._cache)
+        self._ref, self._attn_ref = byref(self._cache), byref(self._attn)
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, kv_heads: int, head_dim: int, device=None):
@@ -219,15 +242,17 @@ class KV4Cache:
         slots (int64; those outside the cache, such as -1, are skipped)."""
         import torch
 
-        kp, ks = _rows(k, v.dtype, self.kv_heads, self.head_dim, "k")
-        vp, vs = _rows(v, v.dtype, self.kv_heads, self.head_dim, "v")
-        if v.dtype not in (torch.float16, torch.float32):
-            raise TypeError(f"k, v: fp16 or fp32 expected, got {v.dtype}")
+        dtype = v.dtype
+        if dtype is not torch.float16 and dtype is not torch.float32:
+            raise TypeError(f"k, v: fp16 or fp32 expected, got {dtype}")
+        kp, ks = _rows(k, dtype, self.kv_heads, self.head_dim, "k")
+        vp, vs = _rows(v, dtype, self.kv_heads, self.head_dim, "v")
         n = k.shape[0]
         if v.shape[0] != n:
             raise ValueError(f"k, v: {n} and {v.shape[0]} rows")
-        check(lib().gsvk_kv4_append(byref(self._cache), kp, ks, vp, vs, v.dtype == torch.float32,
-                                    _vector(slots, torch.int64, n, "slots"), n, _stream(stream)))
+        check(lib().gsvk_kv4_append(self._ref, kp, ks, vp, vs, dtype is torch.float32,
+                                    _vector(slots, torch.int64, n, "slots"), n,
+                                    _stream_for(stream, slots)))
 
     def read(self, slots, k=None, v=None, stream=None):
         """What the slots stand for: fp16 rows k and v [len(slots), kv_heads,
@@ -235,17 +260,20 @@ class KV4Cache:
         import torch
 
         n = slots.numel()
-        shape = (n, self.kv_heads, self.head_dim)
+        sp = _vector(slots, torch.int64, n, "slots")
         if k is None and v is None:
-            k, v = (_new(shape, torch.float16, slots.device, stream) for _ in range(2))
-        ptrs = []
+            k = _kept(torch.empty((n, self.kv_heads, self.head_dim), dtype=torch.float16,
+                                  device=slots.device), stream)
+            v = _kept(torch.empty_like(k), stream)
+        kp = ks = vp = vs = 0
         for t, what in ((k, "k"), (v, "v")):
             if t is not None and t.shape[0] != n:
                 raise ValueError(f"{what}: {n} rows expected, got {t.shape[0]}")
-            ptrs += _rows(t, torch.float16, self.kv_heads, self.head_dim, what) if t is not None \
-                else (None, 0)
-        check(lib().gsvk_kv4_read(byref(self._cache), _vector(slots, torch.int64, n, "slots"), n,
-                                  *ptrs, _stream(stream)))
+        if k is not None:
+            kp, ks = _rows(k, torch.float16, self.kv_heads, self.head_dim, "k")
+        if v is not None:
+            vp, vs = _rows(v, torch.float16, self.kv_heads, self.head_dim, "v")
+        check(lib().gsvk_kv4_read(self._ref, sp, n, kp, ks, vp, vs, _stream_for(stream, slots)))
         return k, v
 
     def attention(self, q, q_start, kv_len, block_table, scale: float, max_q: int, workspace,
@@ -257,27 +285,29 @@ class KV4Cache:
         least these sizes.  Returns fp16 rows like q."""
         import torch
 
-        i32 = torch.int32
+        f16, i32 = torch.float16, torch.int32
         if q.dim() != 3:
             raise ValueError(f"q: [tokens, heads, {self.head_dim}] expected, got {tuple(q.shape)}")
-        n, heads = q.shape[0], q.shape[1]
+        n, heads, _ = q.shape
         a = self._attn
-        a.q, a.q_stride = _rows(q, torch.float16, heads, self.head_dim, "q")
+        a.q, a.q_stride = _rows(q, f16, heads, self.head_dim, "q")
         if out is None:
-            out = _new(q.shape, torch.float16, q.device, stream)
-        elif out.shape != q.shape:
-            raise ValueError(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
-        a.out, a.out_stride = _rows(out, torch.float16, heads, self.head_dim, "out")
-        _tensor(block_table, i32, "block_table", 2)
-        n_seq = block_table.shape[0]
-        a.heads, a.n_tokens, a.n_seq, a.max_blocks = heads, n, n_seq, block_table.shape[1]
-        a.max_q, a.scale = max_q, scale
+            out = _kept(torch.empty((n, heads, self.head_dim), dtype=f16, device=q.device), stream)
+            a.out, a.out_stride = out.data_ptr(), heads * self.head_dim
+        else:
+            if out.shape != q.shape:
+                raise ValueError(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
+            a.out, a.out_stride = _rows(out, f16, heads, self.head_dim, "out")
+        if block_table.dim() != 2:
+            raise ValueError(f"block_table: 2 dimensions expected, got {block_table.dim()}")
+        n_seq, a.max_blocks = block_table.shape
+        a.heads, a.n_tokens, a.n_seq, a.max_q, a.scale = heads, n, n_seq, max_q, scale
         a.q_start = _vector(q_start, i32, n_seq + 1, "q_start")
         a.kv_len = _vector(kv_len, i32, n_seq, "kv_len")
-        a.prefix = _vector(prefix, i32, n_seq, "prefix") if prefix is not None else None
+        a.prefix = None if prefix is None else _vector(prefix, i32, n_seq, "prefix")
         a.block_table = _vector(block_table, i32, 0, "block_table")
         a.workspace, a.workspace_bytes = workspace.ptr, workspace.bytes
-        check(lib().gsvk_kv4_attention(byref(a), _stream(stream)))
+        check(lib().gsvk_kv4_attention(self._attn_ref, _stream_for(stream, q)))
         return out
 
 
@@ -288,21 +318,29 @@ def quantize_rows_i8(x, q=None, scale=None, stream=None):
     takes them."""
     import torch
 
-    if x.dtype not in (torch.float16, torch.float32):
-        raise TypeError(f"x: fp16 or fp32 expected, got {x.dtype}")
-    xp = _tensor(x, x.dtype, "x", 2)
+    dtype = x.dtype
+    if dtype is not torch.float16 and dtype is not torch.float32:
+        raise TypeError(f"x: fp16 or fp32 expected, got {dtype}")
+    xp = _tensor(x, dtype, 2, "x")
     rows, n = x.shape
     if q is None:
-        q = _new((rows, (n + 15) & ~15), torch.int8, x.device, stream)[:, :n]
-    elif tuple(q.shape) != (rows, n):
-        raise ValueError(f"q: {(rows, n)} expected, got {tuple(q.shape)}")
+        ldq = (n + 15) & ~15
+        q = _kept(torch.empty((rows, ldq), dtype=torch.int8, device=x.device), stream)
+        qp = q.data_ptr()
+        if ldq != n:
+            q = q[:, :n]
+    else:
+        if q.shape != x.shape:
+            raise ValueError(f"q: {(rows, n)} expected, got {tuple(q.shape)}")
+        qp = _tensor(q, torch.int8, 2, "q")
+        ldq = _row_stride(q)
     if scale is None:
-        scale = _new((rows,), torch.float32, x.device, stream)
-    check(lib().gsvk_quantize_rows_i8(xp, x.dtype == torch.float32, rows, n, _row_stride(x),
-                                      _tensor(q, torch.int8, "q", 2),
-                                      q.stride(0) if rows > 1 else n,
-                                      _vector(scale, torch.float32, rows, "scale"),
-                                      _stream(stream)))
+        scale = _kept(torch.empty(rows, dtype=torch.float32, device=x.device), stream)
+        sp = scale.data_ptr()
+    else:
+        sp = _vector(scale, torch.float32, rows, "scale")
+    check(lib().gsvk_quantize_rows_i8(xp, dtype is torch.float32, rows, n, _row_stride(x), qp, ldq,
+                                      sp, _stream_for(stream, x)))
     return q, scale
 
 
@@ -313,26 +351,33 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, residual=None, act=ACT_NONE, slop
     where neither is given)."""
     import torch
 
-    ap, bp = _tensor(a, torch.int8, "a", 2), _tensor(b, torch.int8, "b", 2)
+    i8, f32 = torch.int8, torch.float32
+    ap, bp = _tensor(a, i8, 2, "a"), _tensor(b, i8, 2, "b")
     M, K = a.shape
-    N = b.shape[0]
-    if b.shape[1] != K:
-        raise ValueError(f"a, b: rows of {K} and {b.shape[1]}")
-    if c is None and c_f16 is None:
-        c_f16 = _new((M, N), torch.float16, a.device, stream)
-    f32 = torch.float32
-    for t, dt, what in ((c, f32, "c"), (c_f16, torch.float16, "c_f16"), (residual, f32, "residual")):
-        if t is not None:
-            _tensor(t, dt, what, 2)
-            if t.shape[0] != M or t.shape[1] != N:
-                raise ValueError(f"{what}: {(M, N)} expected, got {tuple(t.shape)}")
+    N, kb = b.shape
+    if kb != K:
+        raise ValueError(f"a, b: rows of {K} and {kb}")
+    cp = ldc = hp = ldh = rp = ldr = 0
+    if c is not None:
+        cp, ldc = _matrix(c, f32, M, N, "c")
+    if c_f16 is not None:
+        hp, ldh = _matrix(c_f16, torch.float16, M, N, "c_f16")
+    elif c is None:
+        c_f16 = _kept(torch.empty((M, N), dtype=torch.float16, device=a.device), stream)
+        hp, ldh = c_f16.data_ptr(), N
+    if residual is not None:
+        rp, ldr = _matrix(residual, f32, M, N, "residual")
     g = GemmI8Args(ap, a.stride(0) if M > 1 else K, bp, b.stride(0) if N > 1 else K,
                    _vector(a_scale, f32, M, "a_scale"), _vector(b_scale, f32, N, "b_scale"), M, N, K,
-                   None if bias is None else _vector(bias, f32, N, "bias"),
-                   None if residual is None else residual.data_ptr(),
-                   0 if residual is None else _row_stride(residual),
-                   None if c is None else c.data_ptr(), 0 if c is None else _row_stride(c),
-                   None if c_f16 is None else c_f16.data_ptr(),
-                   0 if c_f16 is None else _row_stride(c_f16), act, slope)
-    check(lib().gsvk_gemm_i8(byref(g), _stream(stream)))
+                   None if bias is None else _vector(bias, f32, N, "bias"), rp, ldr, cp, ldc, hp,
+                   ldh, act, slope)
+    check(lib().gsvk_gemm_i8(byref(g), _stream_for(stream, a)))
     return c if c is not None else c_f16
+
+
+def _matrix(t, dtype, M, N, what):
+    """Address and row stride of an [M, N] tensor."""
+    p = _tensor(t, dtype, 2, what)
+    if t.shape[0] != M or t.shape[1] != N:
+        raise ValueError(f"{what}: {(M, N)} expected, got {tuple(t.shape)}")
+    return p, _row_stride(t)
