@@ -52,20 +52,30 @@ struct AttnArgs {
 // So a code costs 5/8 of an instruction to unpack for the scores, and 3/4 for
 // the values, where two tokens' words are first interleaved by prmt.
 // The weights p_j a_j, scaled by a power of two so that the greatest step seen is
-// at most 1, go in as two fp16 parts, whose sum holds 22 bits: with
-// ROWS = 8 the second part takes the unused rows 8..15 of the same MMA.
+// at most 1, go in as two fp16 parts, whose sum holds 22 bits: up to 8 rows, the
+// second part takes the unused rows 8..15 of the same MMA.
+//
+// Between the products the scores pass through shared memory to a layout with
+// two keys to a lane, so that the softmax costs what the rows there are cost
+// (not the 8 or 16 of an MMA), a key's parameters are converted once, and a
+// maximum is one redux.
 constexpr int kTile = 64;          // keys of a unit
 constexpr int kSplitWarps = 4;     // warps of a CTA
 constexpr int kMaxPieces = 64;     // warps that share an item
 
 template <int HD>
 constexpr int kStages = HD == 32 ? 4 : 3;
-template <int HD>
-constexpr int kCtasPerSm = HD == 128 ? 2 : HD == 64 ? 3 : 4;
+template <int HD, int ROWS>
+constexpr int kCtasPerSm = HD == 128 ? 2 : (HD == 64 ? 3 : 4) - (ROWS == 16);
 template <int HD>
 constexpr int kTileBytes = kTile * (HD + 8);
 template <int HD>
 constexpr int kRecord = HD + 4;  // floats of a joined row: maximum, sum, (pad), values
+// Scores (two keys each, 64 bits) or weights (two fp16 each, first and second part) of a row between
+// the products: 32 pairs, and 32 bytes that keep eight rows off each other's banks.
+constexpr int kRowBytes = 32 * 8 + 32;
+template <int HD, int ROWS>
+constexpr int kWarpBytes = kStages<HD> * kTileBytes<HD> + (ROWS * kRowBytes + 127) / 128 * 128;
 
 // One request's rows and the keys they see.
 struct Request {
@@ -80,29 +90,32 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int s) {
   r.prefix = a.prefix ? a.prefix[s] : 0;
   return r;
 }
-// Keys that row r of a request sees (64-bit on the way: lengths are the caller's).
-__device__ __forceinline__ int limit_of(const AttnArgs& a, const Request& q, int r) {
+// Keys that query row `row` of a request's kv head sees (64-bit on the way: lengths are the caller's).
+__device__ __forceinline__ int limit_of(const AttnArgs& a, const Request& q, int row) {
+  const int r = q.n == 1 || a.group == 1 ? (q.n == 1 ? 0 : row) : row / a.group;
   const long long causal = static_cast<long long>(q.len) - q.n + r + 1;
   const long long see = max(causal, static_cast<long long>(q.prefix));
   const long long have = min(q.len, a.max_blocks << a.shift);
   return static_cast<int>(max(0LL, min(see, have)));
 }
 template <int ROWS>
-__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Request& q, int block) {
-  const int last = min((block + 1) * ROWS, q.n * a.group) - 1;
-  return max(1, (limit_of(a, q, last / a.group) + kTile - 1) / kTile);
-}
-template <int ROWS>
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, const Request& q) {
   return q.n > 0 ? (q.n * a.group + ROWS - 1) / ROWS : 0;
 }
+// Keys that any row of a block sees.
+template <int ROWS>
+__device__ __forceinline__ int keys_of(const AttnArgs& a, const Request& q, int block) {
+  return limit_of(a, q, min((block + 1) * ROWS, q.n * a.group) - 1);
+}
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 // Units of one kv head of a request; *most keeps the longest item.
 template <int ROWS>
 __device__ __forceinline__ long long head_units(const AttnArgs& a, const Request& q, int* most) {
   long long u = 0;
   const int nb = blocks_of<ROWS>(a, q);
+#pragma unroll 1
   for (int b = 0; b < nb; ++b) {
-    const int t = tiles_of<ROWS>(a, q, b);
+    const int t = tiles_of(keys_of<ROWS>(a, q, b));
     u += t;
     *most = max(*most, t);
   }
@@ -113,32 +126,33 @@ __device__ __forceinline__ long long head_units(const AttnArgs& a, const Request
 template <int ROWS>
 struct Cursor {
   Request req;
-  int seq, head, block, tile, tiles, blocks;
+  int seq, head, block, blocks, tile, tiles, keys;
 
-  __device__ void enter(const AttnArgs& a, int s, int h, int b) {
+  __device__ __forceinline__ void set_block(const AttnArgs& a, int b) {
+    block = b;
+    keys = keys_of<ROWS>(a, req, b);
+    tiles = tiles_of(keys);
+  }
+  __device__ __forceinline__ void enter(const AttnArgs& a, int s) {
     seq = s;
     req = request_of(a, s);
     blocks = blocks_of<ROWS>(a, req);
-    head = h;
-    block = b;
-    tile = 0;
-    tiles = blocks > 0 ? tiles_of<ROWS>(a, req, b) : 0;
   }
-  __device__ void next_item(const AttnArgs& a) {
+  __device__ __forceinline__ void next_item(const AttnArgs& a) {
     tile = 0;
-    if (++block < blocks) {
-      tiles = tiles_of<ROWS>(a, req, block);
-      return;
+    if (++block == blocks) {
+      block = 0;
+      if (++head == a.kv_heads) {
+        head = 0;
+        do {
+          if (seq + 1 >= a.n_seq) return;  // the end of the line
+          enter(a, seq + 1);
+        } while (blocks == 0);
+      } else if (blocks == 1) {
+        return;
+      }
     }
-    block = 0;
-    if (++head < a.kv_heads) {
-      if (blocks > 1) tiles = tiles_of<ROWS>(a, req, 0);
-      return;
-    }
-    int s = seq + 1;
-    do {
-      enter(a, min(s, a.n_seq - 1), 0, 0);
-    } while (blocks == 0 && ++s < a.n_seq);
+    set_block(a, block);
   }
 };
 
@@ -150,39 +164,44 @@ __device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, ui
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same without a sum to add to.
+__device__ __forceinline__ void mma_16816_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two weights as fp16, and what that rounding left.
-__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = f2h2(x - f.x, y - f.y);
-}
 
-// The state of ROWS query rows over the tiles seen so far.  Lane (g, t) = (lane / 4, lane % 4) has row g
-// (ROWS = 16: and row g + 8); its part of the sums o is head_dim / 4 dimensions from t head_dim / 4 on.
+// The state of ROWS query rows over the tiles seen so far.  As an MMA operand
+// lane (g, t) = (lane / 4, lane % 4) has row g (ROWS = 16: and row g + 8); its
+// part of the sums o is head_dim / 4 dimensions from t head_dim / 4 on (up to 8 rows: in two
+// parts).  m is the same in every lane; l and pb are a lane's parts of sum p and sum p b.
 template <int HD, int ROWS>
 struct RowState {
-  static constexpr int kR = ROWS / 8;
+  static constexpr int kR = ROWS == 16 ? 2 : 1;
   uint32_t q[HD / 32][2][2 * kR];  // [word][even, odd nibbles][A registers]
   float o[HD / 8][4];
-  float m[kR], l[kR], pb[kR], qsum[kR];
-  float unit;  // weights are held in this power of two
+  float m[ROWS], l[ROWS], pb[ROWS], qsum[ROWS];
+  float unit;  // the weights' power of two
 };
 
 template <int HD, int ROWS>
 __device__ __forceinline__ void load_rows(const AttnArgs& a, const Request& rq, int head, int block, int lane,
                                           RowState<HD, ROWS>& s) {
+  constexpr int kR = RowState<HD, ROWS>::kR;
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int k = 0; k < RowState<HD, ROWS>::kR; ++k) {
+  for (int k = 0; k < kR; ++k) {
     const int row = block * ROWS + 8 * k + g;
-    const bool ok = row < rq.n * a.group;
-    const int r = ok ? row / a.group : 0;
+    const bool ok = 8 * k + g < ROWS && row < rq.n * a.group;
+    const int r = !ok || rq.n == 1 ? 0 : row / a.group;
     const uint16_t* src = a.q + static_cast<size_t>(rq.q0 + r) * a.q_stride +
                           static_cast<size_t>(head * a.group + (row - r * a.group)) * HD + t * (HD / 4);
     float sum = 0.f;
@@ -195,16 +214,22 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, const Request& rq, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += f[i];
       s.q[w][0][k] = __byte_perm(x.x, x.z, 0x5410);
-      s.q[w][0][RowState<HD, ROWS>::kR + k] = __byte_perm(x.y, x.w, 0x5410);
+      s.q[w][0][kR + k] = __byte_perm(x.y, x.w, 0x5410);
       s.q[w][1][k] = __byte_perm(x.x, x.z, 0x7632);
-      s.q[w][1][RowState<HD, ROWS>::kR + k] = __byte_perm(x.y, x.w, 0x7632);
+      s.q[w][1][kR + k] = __byte_perm(x.y, x.w, 0x7632);
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    s.qsum[k] = sum * a.scale_log2;
-    s.m[k] = -INFINITY;
-    s.l[k] = 0.f;
-    s.pb[k] = 0.f;
+    sum *= a.scale_log2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (8 * k + i < ROWS) s.qsum[8 * k + i] = __shfl_sync(0xffffffffu, sum, 4 * i);
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    s.m[r] = -INFINITY;
+    s.l[r] = 0.f;
+    s.pb[r] = 0.f;
   }
 #pragma unroll
   for (int i = 0; i < HD / 8; ++i)
@@ -213,25 +238,23 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, const Request& rq, 
   s.unit = 0.f;
 }
 
-// One tile.  MASK: some of its keys are not seen by some row (limit[k]: keys of the tile that row k sees) or
-// lie in a page that was not loaded (page_ok: a bit for each).
-template <int HD, int ROWS, bool MASK>
-__device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, float scale_log2, const int* limit,
-                                         unsigned page_ok, int lane, RowState<HD, ROWS>& s) {
-  constexpr int kR = ROWS / 8;
+// One tile.  rows: rows of the block; limit: in lane r, the keys of the tile that row r sees; page_ok: a bit for each of
+// the tile's pages that is there.
+template <int HD, int ROWS>
+__device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int sub_shift, float scale_log2, int rows,
+                                         int limit, unsigned page_ok, int lane, RowState<HD, ROWS>& s) {
+  constexpr int kR = RowState<HD, ROWS>::kR;
   const int g = lane >> 2, t = lane & 3;
-  const int sub_bytes = kv4_head_bytes(sub_shift, HD);
-  const int krow = (g >> 1) + 4 * (g & 1);  // column g of a score MMA is this key of its eight
-  float z[kTile / 8][2 * kR];
-  float top[kR];
-#pragma unroll
-  for (int k = 0; k < kR; ++k) top[k] = s.m[k];
+  const int sub_bytes = kv4_head_bytes(sub_shift, HD), sub_mask = (1 << sub_shift) - 1;
+  // ------------------------------------------------------------------ scores
+  // Column g of a score MMA over keys 8 i .. 8 i + 7 is key 8 i + g / 2 + 4 (g % 2), so lane (g, t) gets keys
+  // 8 i + t and 8 i + 4 + t, the pair that the value MMA wants of it; pair (i, t) lies at place
+  // 8 (i / 2) + 2 t + i % 2 of a row.
 #pragma unroll
   for (int i = 0; i < kTile / 8; ++i) {
-    const int j0 = 8 * i, sub = j0 >> sub_shift, at = j0 & ((1 << sub_shift) - 1);
-    const uint8_t* b = tile + sub * sub_bytes;
+    const int j = 8 * i + (g >> 1) + 4 * (g & 1);
+    const uint8_t* src = tile + (j >> sub_shift) * sub_bytes + (j & sub_mask) * (HD / 2) + t * (HD / 8);
     uint32_t w[HD / 32];
-    const uint8_t* src = b + (at + krow) * (HD / 2) + t * (HD / 8);
     if constexpr (HD == 32) {
       w[0] = *reinterpret_cast<const uint32_t*>(src);
     } else if constexpr (HD == 64) {
@@ -241,74 +264,91 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, flo
       const uint4 v = *reinterpret_cast<const uint4*>(src);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
-    float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+    float even[4], odd[4];
 #pragma unroll
     for (int u = 0; u < HD / 32; ++u) {
       const uint32_t x = w[u], y = x >> 8;
-      const uint32_t* q0 = s.q[u][0];
-      const uint32_t* q1 = s.q[u][1];
-      if constexpr (ROWS == 8) {
-        mma_16816(even, q0[0], 0u, q0[1], 0u, x & 0x000f000fu, y & 0x000f000fu);
-        mma_16816(odd, q1[0], 0u, q1[1], 0u, x & 0x00f000f0u, y & 0x00f000f0u);
+      const uint32_t *q0 = s.q[u][0], *q1 = s.q[u][1];
+      const uint32_t e1 = kR == 2 ? q0[1] : 0u, e2 = q0[kR], e3 = kR == 2 ? q0[3 % (2 * kR)] : 0u;
+      const uint32_t o1 = kR == 2 ? q1[1] : 0u, o2 = q1[kR], o3 = kR == 2 ? q1[3 % (2 * kR)] : 0u;
+      if (u == 0) {
+        mma_16816_first(even, q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
+        mma_16816_first(odd, q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
       } else {
-        mma_16816(even, q0[0], q0[1], q0[2], q0[3], x & 0x000f000fu, y & 0x000f000fu);
-        mma_16816(odd, q1[0], q1[1], q1[2], q1[3], x & 0x00f000f0u, y & 0x00f000f0u);
+        mma_16816(even, q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
+        mma_16816(odd, q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
       }
     }
-    // this lane's two keys of the eight: t and 4 + t
-    const uint8_t* par = b + kv4_k_par(sub_shift, HD) + (at + t) * 4;
+    const int place = 8 * (i >> 1) + 2 * t + (i & 1);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const __half2 h = *reinterpret_cast<const __half2*>(par + 16 * c);
-      const float2 f = __half22float2(h);
-      const float step = f.x * (scale_log2 * 16777216.f);
-#pragma unroll
-      for (int k = 0; k < kR; ++k) {
-        float v = fmaf(fmaf(odd[2 * k + c], 0.0625f, even[2 * k + c]), step, f.y * s.qsum[k]);
-        if constexpr (MASK) {
-          const int j = j0 + 4 * c + t;
-          if (j >= limit[k] || !(page_ok >> sub & 1u)) v = -INFINITY;
-        }
-        z[i][2 * k + c] = v;
-        top[k] = fmaxf(top[k], v);
-      }
-    }
+    for (int k = 0; k < kR; ++k)
+      if (ROWS >= 8 || g < ROWS)
+        *reinterpret_cast<float2*>(mid + (8 * k + g) * kRowBytes + place * 8) =
+            make_float2(fmaf(odd[2 * k], 0.0625f, even[2 * k]), fmaf(odd[2 * k + 1], 0.0625f, even[2 * k + 1]));
   }
-  // the greatest step among the tile's values sets the unit of the weights
+  // ----------------------------------------------------------------- softmax
+  // This lane's keys: pair (i, t) = (lane / 4, lane % 4), the lane's place in a row likewise.
+  const int j0 = 8 * g + t, sub0 = j0 >> sub_shift;  // the second key, 4 on, has the same page
+  const uint8_t* par = tile + sub0 * sub_bytes + (j0 & sub_mask) * 4;
+  const bool here = page_ok >> sub0 & 1u;
+  const uint32_t kp0 = *reinterpret_cast<const uint32_t*>(par + kv4_k_par(sub_shift, HD));
+  const uint32_t kp1 = *reinterpret_cast<const uint32_t*>(par + kv4_k_par(sub_shift, HD) + 16);
+  const uint32_t vp0 = *reinterpret_cast<const uint32_t*>(par + kv4_v_par(sub_shift, HD));
+  const uint32_t vp1 = *reinterpret_cast<const uint32_t*>(par + kv4_v_par(sub_shift, HD) + 16);
+  int any = __shfl_sync(0xffffffffu, limit, rows - 1);
+  if (!here) any = 0;
+  // the greatest step among the values that any row sees sets the unit of the weights
   uint32_t most = 0;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int j = lane + 32 * c, sub = j >> sub_shift, at = j & ((1 << sub_shift) - 1);
-    uint32_t h = *reinterpret_cast<const uint16_t*>(tile + sub * sub_bytes + kv4_v_par(sub_shift, HD) + at * 4);
-    if constexpr (MASK) {
-      if (j >= limit[kR] || !(page_ok >> sub & 1u)) h = 0;  // limit[kR]: keys that any row sees
-    }
-    if (h < 0x7c00u) most = max(most, h);
-  }
+  if (j0 < any && (vp0 & 0xffffu) < 0x7c00u) most = vp0 & 0xffffu;
+  if (j0 + 4 < any && (vp1 & 0xffffu) < 0x7c00u) most = max(most, vp1 & 0xffffu);
   most = __reduce_max_sync(0xffffffffu, most);
-  // the power of two above the step: its fp32 exponent, plus one
+  // the power of two above it: its fp32 exponent, plus one
   const float step_unit =
       __uint_as_float((__float_as_uint(h2f(static_cast<uint16_t>(most))) & 0x7f800000u) + 0x00800000u);
   const float unit = most ? fmaxf(s.unit, step_unit) : s.unit;
   const float per_unit = unit > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;  // 1 / unit
   const float rescale = s.unit * per_unit;
   s.unit = unit;
+  const float a0 = h2f(static_cast<uint16_t>(kp0)) * (scale_log2 * 16777216.f), b0 = h2f(static_cast<uint16_t>(kp0 >> 16));
+  const float a1 = h2f(static_cast<uint16_t>(kp1)) * (scale_log2 * 16777216.f), b1 = h2f(static_cast<uint16_t>(kp1 >> 16));
+  const float st0 = h2f(static_cast<uint16_t>(vp0)) * per_unit, low0 = h2f(static_cast<uint16_t>(vp0 >> 16));
+  const float st1 = h2f(static_cast<uint16_t>(vp1)) * per_unit, low1 = h2f(static_cast<uint16_t>(vp1 >> 16));
+  const int place = 8 * (g >> 1) + 2 * t + (g & 1);
+  __syncwarp();
   float fix[kR];
   bool changed = rescale != 1.f;
 #pragma unroll
-  for (int k = 0; k < kR; ++k) {
-    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
-    const float base = top[k] == -INFINITY ? 0.f : top[k];
-    const float keep = ex2(s.m[k] - base);
+  for (int k = 0; k < kR; ++k) fix[k] = rescale;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (ROWS > 1 && r >= rows) break;
+    uint8_t* at = mid + r * kRowBytes + place * 8;
+    const float2 z = *reinterpret_cast<const float2*>(at);
+    const int lim = __shfl_sync(0xffffffffu, limit, r);
+    const bool see0 = here && j0 < lim, see1 = here && j0 + 4 < lim;
+    const float z0 = see0 ? fmaf(z.x, a0, b0 * s.qsum[r]) : -INFINITY;
+    const float z1 = see1 ? fmaf(z.y, a1, b1 * s.qsum[r]) : -INFINITY;
+    const float top = fmaxf(s.m[r], warp_max(fmaxf(z0, z1)));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float keep = ex2(s.m[r] - base);
+    s.m[r] = top;
+    const float p0 = ex2(z0 - base), p1 = ex2(z1 - base);
+    s.l[r] = fmaf(s.l[r], keep, p0 + p1);
+    // a key that is not seen has p = 0, whatever its parameters
+    s.pb[r] = fmaf(s.pb[r], keep, (see0 ? p0 * low0 : 0.f) + (see1 ? p1 * low1 : 0.f));
+    const float w0 = see0 ? p0 * st0 : 0.f, w1 = see1 ? p1 * st1 : 0.f;
+    const __half2 h = __floats2half2_rn(w0, w1);
+    const float2 f = __half22float2(h);
+    *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&h), f2h2(w0 - f.x, w1 - f.y));
     changed |= keep != 1.f;
-    s.m[k] = top[k];
-    s.l[k] *= keep;
-    s.pb[k] *= keep;
-    fix[k] = keep * rescale;
-    top[k] = base;
+    if (r < 8) {
+      if (g == r) fix[0] = keep * rescale;
+    } else {
+      if (g == r - 8) fix[kR - 1] = keep * rescale;
+    }
   }
-  if (__any_sync(0xffffffffu, changed)) {
+  __syncwarp();
+  if (changed) {  // the same in every lane
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
       s.o[i][0] *= fix[0];
@@ -317,43 +357,22 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, flo
       s.o[i][3] *= fix[kR - 1];
     }
   }
+  // ------------------------------------------------------------------ values
 #pragma unroll
   for (int i = 0; i < kTile / 16; ++i) {
-    const int j0 = 16 * i, sub = j0 >> sub_shift, at = j0 & ((1 << sub_shift) - 1);
-    const uint8_t* b = tile + sub * sub_bytes;
-    const uint8_t* par = b + kv4_v_par(sub_shift, HD) + (at + t) * 4;
-    uint32_t hi[kR][2], lo[kR][2];
+    // [row][key pair 16 i + t + {0, 4}, 16 i + 8 + t + {0, 4}]: first part, second part of each
+    uint4 w[kR];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {  // keys 8 c + t and 8 c + 4 + t
-      float wt[kR][2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const __half2 h = *reinterpret_cast<const __half2*>(par + 32 * c + 16 * e);
-        const float2 f = __half22float2(h);
-        const float step = f.x * per_unit;
-#pragma unroll
-        for (int k = 0; k < kR; ++k) {
-          const float v = z[2 * i + c][2 * k + e];
-          float p = ex2(v - top[k]);
-          float low = f.y, st = step;
-          if constexpr (MASK) {
-            const int j = j0 + 8 * c + 4 * e + t;
-            if (j >= limit[k] || !(page_ok >> sub & 1u)) p = low = st = 0.f;
-          }
-          s.l[k] += p;
-          s.pb[k] = fmaf(p, low, s.pb[k]);
-          wt[k][e] = p * st;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kR; ++k) split2(wt[k][0], wt[k][1], &hi[k][c], &lo[k][c]);
+    for (int k = 0; k < kR; ++k) {
+      w[k] = make_uint4(0, 0, 0, 0);
+      if (8 * k + g < rows) w[k] = *reinterpret_cast<const uint4*>(mid + (8 * k + g) * kRowBytes + (8 * i + 2 * t) * 8);
     }
-    const auto add = [&](int n, uint32_t b0, uint32_t b1) {
-      if constexpr (ROWS == 8) {
-        mma_16816(s.o[n], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
+    const auto add = [&](int n, uint32_t x, uint32_t y) {
+      if constexpr (kR == 1) {
+        mma_16816(s.o[n], w[0].x, w[0].y, w[0].z, w[0].w, x, y);
       } else {
-        mma_16816(s.o[n], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-        mma_16816(s.o[n], lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
+        mma_16816(s.o[n], w[0].x, w[kR - 1].x, w[0].z, w[kR - 1].z, x, y);
+        mma_16816(s.o[n], w[0].y, w[kR - 1].y, w[0].w, w[kR - 1].w, x, y);
       }
     };
     const auto four = [&](int n, uint32_t x, uint32_t y) {  // four nibbles of two pairs of tokens
@@ -363,7 +382,8 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, flo
       add(n + 2, x & 0x000f000fu, y & 0x000f000fu);
       add(n + 3, x & 0x00f000f0u, y & 0x00f000f0u);
     };
-    const uint8_t* src = b + kv4_v_codes(sub_shift, HD) + (at + t) * (HD / 2);
+    const int j = 16 * i + t;
+    const uint8_t* src = tile + (j >> sub_shift) * sub_bytes + kv4_v_codes(sub_shift, HD) + (j & sub_mask) * (HD / 2);
     if constexpr (HD == 32) {
       uint32_t x[4];
 #pragma unroll
@@ -390,22 +410,23 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, int sub_shift, flo
 
 // Where query row `row` of a request's kv head goes.
 __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, const Request& rq, int head, int row, int hd) {
-  const int r = row / a.group;
+  const int r = rq.n == 1 ? 0 : row / a.group;
   return a.out + static_cast<size_t>(rq.q0 + r) * a.out_stride +
          static_cast<size_t>(head * a.group + row - r * a.group) * hd;
 }
 
 // Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.
 template <int HD, int ROWS>
-__device__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int block, int first, int last, int lane) {
+__device__ __forceinline__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int block, int first, int last,
+                                            int lane) {
   constexpr int kD = HD / 32;
-  const int rows = min(ROWS, rq.n * a.group - block * ROWS);
+  const int rows = min(ROWS, rq.n * a.group - block * ROWS), n = last - first + 1;
   const size_t stride = static_cast<size_t>(2) * ROWS * kRecord<HD>;  // from a warp's records to the next's
+#pragma unroll 1
   for (int row = 0; row < rows; ++row) {
     // the first warp's piece is its last one (second record), the others' their first
     const float* r0 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + ROWS + row) * kRecord<HD>;
     const float* r1 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + row) * kRecord<HD>;
-    const int n = last - first + 1;
     float top = -INFINITY;
     for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? r1 + i * stride : r0)[0]);
     top = warp_max(top);
@@ -428,118 +449,121 @@ __device__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int 
 }
 
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_split_kernel(const AttnArgs a) {
-  constexpr int kR = ROWS / 8;
+__global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_attn_split_kernel(const AttnArgs a) {
+  constexpr int kR = RowState<HD, ROWS>::kR;
   constexpr int kS = kStages<HD>;
   constexpr int kThreads = kSplitWarps * 32;
   extern __shared__ __align__(128) uint8_t split_smem[];
   __shared__ uint64_t bars[kSplitWarps][kS];
   __shared__ long long s_before[kThreads + 1];
+  __shared__ long long s_share;
   __shared__ int s_most;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint8_t* ring = split_smem + warp * kS * kTileBytes<HD>;
+  uint8_t* ring = split_smem + warp * kWarpBytes<HD, ROWS>;
+  uint8_t* mid = ring + kS * kTileBytes<HD>;
+  const int warps = static_cast<int>(gridDim.x) * kSplitWarps;
 
   // the line of units: each thread sums a run of requests
   const int per = (a.n_seq + kThreads - 1) / kThreads;
   if (tid == 0) s_most = 0;
   if (lane < kS) mbar_init(&bars[warp][lane], 1);
   fence_barrier_init();
-  __syncthreads();
+  long long inc = 0;
   {
-    long long mine = 0;
     int most = 0;
     for (int s = tid * per; s < min((tid + 1) * per, a.n_seq); ++s)
-      mine += a.kv_heads * head_units<ROWS>(a, request_of(a, s), &most);
-    atomicMax(&s_most, most);
-    long long inc = mine;
+      inc += a.kv_heads * head_units<ROWS>(a, request_of(a, s), &most);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();  // s_most is there
+    if (lane == 0) atomicMax(&s_most, most);
     s_before[tid + 1] = inc;
     __syncthreads();
-    long long add = 0;
-    for (int w = 0; w < warp; ++w) add += s_before[32 * (w + 1)];
+    for (int w = 0; w < warp; ++w) inc += s_before[32 * (w + 1)];
     __syncthreads();
-    s_before[tid + 1] = inc + add;
+    s_before[tid + 1] = inc;
     if (tid == 0) s_before[0] = 0;
+    if (tid == kThreads - 1)
+      // a run: an equal share, and no less than lets kMaxPieces warps cover the longest item
+      s_share = max((inc + warps - 1) / warps, static_cast<long long>((s_most + kMaxPieces - 1) / kMaxPieces));
     __syncthreads();
   }
   const long long total = s_before[kThreads];
-  const int warps = static_cast<int>(gridDim.x) * kSplitWarps;
   const int me = static_cast<int>(blockIdx.x) * kSplitWarps + warp;
-  // a run: an equal share, and no less than lets kMaxPieces warps cover the longest item
-  const long long share = max((total + warps - 1) / warps, static_cast<long long>((s_most + kMaxPieces - 1) / kMaxPieces));
-  const long long u0 = me * share, u1 = min(total, u0 + share);
+  const long long u0 = me * s_share, u1 = min(total, u0 + s_share);
   if (u0 >= u1) return;
+  // from here on units count from u0: a run has fewer than 2^31
+  const int share = static_cast<int>(s_share);
+  const int run = static_cast<int>(u1 - u0);
 
   // the request that holds unit u0, then the head, block and tile
   Cursor<ROWS> at;
-  long long item_start;  // unit of the current item's tile 0
   {
     int lo = 0, hi = kThreads;  // the last run of requests that starts at or before u0
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_before[mid] <= u0) {
-        lo = mid;
+      const int m = (lo + hi) >> 1;
+      if (s_before[m] <= u0) {
+        lo = m;
       } else {
-        hi = mid;
+        hi = m;
       }
     }
     long long left = u0 - s_before[lo];
     int s = lo * per, most = 0;
     long long u = 1;
+#pragma unroll 1
     for (;; s += 32) {  // a lane to a request of the run
       const long long mine = s + lane < a.n_seq ? head_units<ROWS>(a, request_of(a, s + lane), &most) : 0;
-      long long inc = mine;
+      long long sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
       }
-      const unsigned here = __ballot_sync(0xffffffffu, left < inc * a.kv_heads);
-      if (here) {
-        const int i = __ffs(static_cast<int>(here)) - 1;
+      const unsigned found = __ballot_sync(0xffffffffu, left < sum * a.kv_heads);
+      if (found) {
+        const int i = __ffs(static_cast<int>(found)) - 1;
         s += i;
         u = __shfl_sync(0xffffffffu, mine, i);
-        left -= __shfl_sync(0xffffffffu, inc - mine, i) * a.kv_heads;
+        left -= __shfl_sync(0xffffffffu, sum - mine, i) * a.kv_heads;
         break;
       }
-      left -= __shfl_sync(0xffffffffu, inc, 31) * a.kv_heads;
+      left -= __shfl_sync(0xffffffffu, sum, 31) * a.kv_heads;
       if (s + 32 >= a.n_seq) return;  // not reached: u0 lies on the line
     }
-    const int head = static_cast<int>(left / u);
-    left -= head * u;
-    at.enter(a, s, head, 0);
+    // left < kv_heads units of a request
+    at.head = (u >> 31) == 0 && (left >> 31) == 0 ? static_cast<int>(left) / static_cast<int>(u) : static_cast<int>(left / u);
+    left -= at.head * u;
+    at.enter(a, s);
+    at.set_block(a, 0);
     while (left >= at.tiles && at.block + 1 < at.blocks) {
       left -= at.tiles;
-      at.tiles = tiles_of<ROWS>(a, at.req, ++at.block);
+      at.set_block(a, at.block + 1);
     }
     at.tile = static_cast<int>(left);
-    item_start = u0 - left;
   }
+  int item_start = -at.tile;  // the item's tile 0, counted from u0
 
   const int sub_shift = min(a.shift, 6), subs = kTile >> sub_shift;  // pages of a tile, or parts of one
   // The copies run kS tiles ahead of the sums; the page of the next copy is
   // read one tile earlier still, so that nothing waits for it.
   Cursor<ROWS> ahead = at;
-  long long to_load = u1 - u0;
+  int to_load = run;
   int page = -1;
+  unsigned ok_bits = 0;  // 8 bits for each stage: pages that are there
   const auto fetch_page = [&]() {
-    page = -1;
-    if (to_load > 0 && lane < subs) {
-      const int last = min((ahead.block + 1) * ROWS, ahead.req.n * a.group) - 1;
-      const int j = ahead.tile * kTile + (lane << sub_shift);
-      if (j < limit_of(a, ahead.req, last / a.group))
-        page = a.table[static_cast<size_t>(ahead.seq) * a.max_blocks + (j >> a.shift)];
-    }
+    const int j = ahead.tile * kTile + (lane << sub_shift);
+    page = lane < subs && j < ahead.keys ? a.table[static_cast<size_t>(ahead.seq) * a.max_blocks + (j >> a.shift)] : -1;
   };
-  unsigned ok_bits[kS];
-  const auto issue = [&](int stage, uint64_t* bar) -> unsigned {
+  const auto issue = [&](int stage) {
     const bool ok = page >= 0 && page < a.n_pages;
     const unsigned mask = __ballot_sync(0xffffffffu, ok);
     const int bytes = kv4_head_bytes(sub_shift, HD);
+    uint64_t* bar = &bars[warp][stage];
     if (lane == 0) mbar_arrive_expect_tx(bar, __popc(mask) * bytes);
     __syncwarp();
     if (ok) {
@@ -557,60 +581,39 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_spl
         bulk_load(dst + kv4_v_par(6, HD), src + kv4_v_par(7, HD) + half * 256, 256, bar);
       }
     }
-    --to_load;
-    if (to_load > 0) {
+    ok_bits = (ok_bits & ~(0xffu << (8 * stage))) | mask << (8 * stage);
+    if (--to_load > 0) {
       if (++ahead.tile == ahead.tiles) ahead.next_item(a);
       fetch_page();
     }
-    return mask;
   };
   fetch_page();
-#pragma unroll
-  for (int st = 0; st < kS; ++st) ok_bits[st] = to_load > 0 ? issue(st, &bars[warp][st]) : 0u;
+#pragma unroll 1
+  for (int st = 0; st < kS; ++st)
+    if (to_load > 0) issue(st);
 
   RowState<HD, ROWS> s;
   int stage = 0;
   uint32_t parity = 0;
-  long long u = u0;
+  int u = 0;
   bool alive = true;
-  while (u < u1) {
-    const int t1 = static_cast<int>(min(static_cast<long long>(at.tiles), at.tile + (u1 - u)));
+#pragma unroll 1
+  while (u < run) {
+    const int t1 = min(at.tiles, at.tile + (run - u));
     load_rows<HD, ROWS>(a, at.req, at.head, at.block, lane, s);
-    int limit[kR + 1];
-    int least = 0x7fffffff;
-    {
-      const int rows = at.req.n * a.group, row0 = at.block * ROWS;
-      least = limit_of(a, at.req, row0 / a.group);
-#pragma unroll
-      for (int k = 0; k < kR; ++k)
-        limit[k] = limit_of(a, at.req, min(row0 + 8 * k + (lane >> 2), rows - 1) / a.group);
-      limit[kR] = limit_of(a, at.req, (min(row0 + ROWS, rows) - 1) / a.group);
-    }
+    const int all = at.req.n * a.group, rows = min(ROWS, all - at.block * ROWS);
+    const int limit = limit_of(a, at.req, min(at.block * ROWS + lane, all - 1));  // of row `lane`
+#pragma unroll 1
     for (int tile = at.tile; tile < t1; ++tile, ++u) {
       if (alive) alive = mbar_wait(&bars[warp][stage], parity, a.status);
       if (!__all_sync(0xffffffffu, alive)) {
         alive = false;
         break;
       }
-      unsigned ok = 0;
-#pragma unroll
-      for (int st = 0; st < kS; ++st) ok = st == stage ? ok_bits[st] : ok;
-      const uint8_t* buf = ring + stage * kTileBytes<HD>;
-      const int j0 = tile * kTile;
-      if (j0 + kTile <= least && ok == (1u << subs) - 1u) {
-        add_tile<HD, ROWS, false>(buf, sub_shift, a.scale_log2, nullptr, 0, lane, s);
-      } else {
-        int rel[kR + 1];
-#pragma unroll
-        for (int k = 0; k <= kR; ++k) rel[k] = limit[k] - j0;
-        add_tile<HD, ROWS, true>(buf, sub_shift, a.scale_log2, rel, ok, lane, s);
-      }
+      add_tile<HD, ROWS>(ring + stage * kTileBytes<HD>, mid, sub_shift, a.scale_log2, rows, limit - tile * kTile,
+                         ok_bits >> (8 * stage), lane, s);
       __syncwarp();  // every lane has read the tile
-      if (to_load > 0) {
-        const unsigned got = issue(stage, &bars[warp][stage]);
-#pragma unroll
-        for (int st = 0; st < kS; ++st) ok_bits[st] = st == stage ? got : ok_bits[st];
-      }
+      if (to_load > 0) issue(stage);
       if (++stage == kS) {
         stage = 0;
         parity ^= 1u;
@@ -619,28 +622,33 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_spl
     if (!alive) break;
     // the item's rows so far: sums over the lanes of a row, and the codes' unit
     const bool whole = at.tile == 0 && t1 == at.tiles;
-    const int first = static_cast<int>(item_start / share), last = static_cast<int>((item_start + at.tiles - 1) / share);
+    // the warps that share the item
+    const int first = me - (item_start < 0 ? (share - 1 - item_start) / share : 0);
+    const int last = me + (item_start + at.tiles - 1) / share;
     const float up = s.unit * 16777216.f;
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
-      float l = s.l[k], pb = s.pb[k];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      pb += __shfl_xor_sync(0xffffffffu, pb, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      pb += __shfl_xor_sync(0xffffffffu, pb, 2);
+      float l = 0.f, pb = 0.f, m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (8 * k + i < ROWS && 8 * k + i < rows) {
+          const float sum = warp_sum(s.l[(8 * k + i) % ROWS]), low = warp_sum(s.pb[(8 * k + i) % ROWS]);
+          if ((lane >> 2) == i) l = sum, pb = low, m = s.m[(8 * k + i) % ROWS];
+        }
+      }
       const int in_block = 8 * k + (lane >> 2), row = at.block * ROWS + in_block;
-      if (row < at.req.n * a.group) {
+      if (in_block < rows) {
         float v[HD / 4];
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float sum = ROWS == 8 ? s.o[i][c] + s.o[i][2 + c] : s.o[i][2 * k + c];
+            const float sum = kR == 1 ? s.o[i][c] + s.o[i][2 + c] : s.o[i][2 * k + c];
             v[c * (HD / 8) + i] = fmaf(sum, (i & 1) ? up * 0.0625f : up, pb);
           }
         if (whole) {
           uint16_t* o = out_row(a, at.req, at.head, row, HD) + (lane & 3) * (HD / 4);
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = 1.f / l;
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) {
             uint32_t h[4];
@@ -651,7 +659,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_spl
           }
         } else {
           float* r = a.parts + (static_cast<size_t>(me) * 2 * ROWS + (me == first ? ROWS : 0) + in_block) * kRecord<HD>;
-          if ((lane & 3) == 0) *reinterpret_cast<float2*>(r) = make_float2(s.m[k], l);
+          if ((lane & 3) == 0) *reinterpret_cast<float2*>(r) = make_float2(m, l);
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i)
             *reinterpret_cast<float4*>(r + 4 + (lane & 3) * (HD / 4) + 4 * i) =
@@ -672,7 +680,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_spl
       }
     }
     item_start += at.tiles;
-    if (u < u1) at.next_item(a);
+    if (u < run) at.next_item(a);
   }
   if (!alive) {  // a copy never came: leave once those in flight have landed, as far as waits go
     for (int st = 0; st < kS; ++st) mbar_wait(&bars[warp][st], parity ^ (st < stage ? 1u : 0u), a.status);
@@ -681,7 +689,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD>) kv4_attn_spl
 
 template <int HD, int ROWS>
 int launch_split(const AttnArgs& a, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(kSplitWarps) * kStages<HD> * kTileBytes<HD>;
+  const size_t smem = static_cast<size_t>(kSplitWarps) * kWarpBytes<HD, ROWS>;
   static bool ready[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -694,13 +702,13 @@ int launch_split(const AttnArgs& a, cudaStream_t st) {
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   kv4_attn_split_kernel<HD, ROWS>
-      <<<static_cast<unsigned>(sm_count() * kCtasPerSm<HD>), kSplitWarps * 32, smem, st>>>(a);
+      <<<static_cast<unsigned>(sm_count() * kCtasPerSm<HD, ROWS>), kSplitWarps * 32, smem, st>>>(a);
   return check_launch("kv4_attn_split_kernel");
 }
 
 // Tickets (zero between calls), then the records.
 size_t split_warps(size_t hd) {
-  return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128> : hd == 64 ? kCtasPerSm<64> : kCtasPerSm<32>);
+  return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
 }
 size_t tickets_bytes(size_t hd) { return (split_warps(hd) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
 
@@ -769,11 +777,15 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + tickets_bytes(hd));
   a.status = device_status();
   cudaStream_t st = as_cuda(stream);
-  // up to 8 rows to a kv head leave half of an MMA's rows to the weights' second parts
-  if (g->max_q * a.group <= 8) {
-    return hd == 32 ? launch_split<32, 8>(a, st) : hd == 64 ? launch_split<64, 8>(a, st) : launch_split<128, 8>(a, st);
-  }
-  return hd == 32 ? launch_split<32, 16>(a, st) : hd == 64 ? launch_split<64, 16>(a, st) : launch_split<128, 16>(a, st);
+  // as few MMA and softmax rows as the requests' tokens need
+  const size_t rows = g->max_q * a.group;
+  const auto run = [&](auto launch32, auto launch64, auto launch128) {
+    return hd == 32 ? launch32(a, st) : hd == 64 ? launch64(a, st) : launch128(a, st);
+  };
+  if (rows <= 1) return run(launch_split<32, 1>, launch_split<64, 1>, launch_split<128, 1>);
+  if (rows <= 4) return run(launch_split<32, 4>, launch_split<64, 4>, launch_split<128, 4>);
+  if (rows <= 8) return run(launch_split<32, 8>, launch_split<64, 8>, launch_split<128, 8>);
+  return run(launch_split<32, 16>, launch_split<64, 16>, launch_split<128, 16>);
 }
 
 }  // extern "C"
