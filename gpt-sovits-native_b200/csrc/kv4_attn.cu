@@ -63,10 +63,10 @@ constexpr int kTile = 64;          // keys of a unit
 constexpr int kSplitWarps = 4;     // warps of a CTA
 constexpr int kMaxPieces = 64;     // warps that share an item
 
-template <int HD>
-constexpr int kStages = HD == 32 ? 4 : 3;
 template <int HD, int ROWS>
 constexpr int kCtasPerSm = HD == 128 ? 2 : (HD == 64 ? 3 : 4) - (ROWS == 16);
+template <int HD, int ROWS>
+constexpr int kStages = HD == 32 ? 4 : 3;
 template <int HD>
 constexpr int kTileBytes = kTile * (HD + 8);
 template <int HD>
@@ -75,7 +75,7 @@ constexpr int kRecord = HD + 4;  // floats of a joined row: maximum, sum, (pad),
 // the products: 32 pairs, and 32 bytes that keep eight rows off each other's banks.
 constexpr int kRowBytes = 32 * 8 + 32;
 template <int HD, int ROWS>
-constexpr int kWarpBytes = kStages<HD> * kTileBytes<HD> + (ROWS * kRowBytes + 127) / 128 * 128;
+constexpr int kWarpBytes = kStages<HD, ROWS> * kTileBytes<HD> + (ROWS * kRowBytes + 127) / 128 * 128;
 
 // One request's rows and the keys they see.
 struct Request {
@@ -158,8 +158,7 @@ struct Cursor {
 
 __device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -167,8 +166,7 @@ __device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, ui
 // The same without a sum to add to.
 __device__ __forceinline__ void mma_16816_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                 uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -250,41 +248,52 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   // Column g of a score MMA over keys 8 i .. 8 i + 7 is key 8 i + g / 2 + 4 (g % 2), so lane (g, t) gets keys
   // 8 i + t and 8 i + 4 + t, the pair that the value MMA wants of it; pair (i, t) lies at place
   // 8 (i / 2) + 2 t + i % 2 of a row.
+  constexpr int kSide = HD / 32;  // MMAs of several eights of keys side by side: each waits for its own last one only
 #pragma unroll
-  for (int i = 0; i < kTile / 8; ++i) {
-    const int j = 8 * i + (g >> 1) + 4 * (g & 1);
-    const uint8_t* src = tile + (j >> sub_shift) * sub_bytes + (j & sub_mask) * (HD / 2) + t * (HD / 8);
-    uint32_t w[HD / 32];
-    if constexpr (HD == 32) {
-      w[0] = *reinterpret_cast<const uint32_t*>(src);
-    } else if constexpr (HD == 64) {
-      const uint2 v = *reinterpret_cast<const uint2*>(src);
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(src);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  for (int i0 = 0; i0 < kTile / 8; i0 += kSide) {
+    uint32_t w[kSide][HD / 32];
+    float even[kSide][4], odd[kSide][4];
+#pragma unroll
+    for (int i = 0; i < kSide; ++i) {
+      const int j = 8 * (i0 + i) + (g >> 1) + 4 * (g & 1);
+      const uint8_t* src = tile + (j >> sub_shift) * sub_bytes + (j & sub_mask) * (HD / 2) + t * (HD / 8);
+      if constexpr (HD == 32) {
+        w[i][0] = *reinterpret_cast<const uint32_t*>(src);
+      } else if constexpr (HD == 64) {
+        const uint2 v = *reinterpret_cast<const uint2*>(src);
+        w[i][0] = v.x, w[i][1] = v.y;
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(src);
+        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+      }
     }
-    float even[4], odd[4];
 #pragma unroll
     for (int u = 0; u < HD / 32; ++u) {
-      const uint32_t x = w[u], y = x >> 8;
       const uint32_t *q0 = s.q[u][0], *q1 = s.q[u][1];
       const uint32_t e1 = kR == 2 ? q0[1] : 0u, e2 = q0[kR], e3 = kR == 2 ? q0[3 % (2 * kR)] : 0u;
       const uint32_t o1 = kR == 2 ? q1[1] : 0u, o2 = q1[kR], o3 = kR == 2 ? q1[3 % (2 * kR)] : 0u;
-      if (u == 0) {
-        mma_16816_first(even, q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
-        mma_16816_first(odd, q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
-      } else {
-        mma_16816(even, q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
-        mma_16816(odd, q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
+#pragma unroll
+      for (int i = 0; i < kSide; ++i) {
+        const uint32_t x = w[i][u], y = x >> 8;
+        if (u == 0) {
+          mma_16816_first(even[i], q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
+          mma_16816_first(odd[i], q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
+        } else {
+          mma_16816(even[i], q0[0], e1, e2, e3, x & 0x000f000fu, y & 0x000f000fu);
+          mma_16816(odd[i], q1[0], o1, o2, o3, x & 0x00f000f0u, y & 0x00f000f0u);
+        }
       }
     }
-    const int place = 8 * (i >> 1) + 2 * t + (i & 1);
 #pragma unroll
-    for (int k = 0; k < kR; ++k)
-      if (ROWS >= 8 || g < ROWS)
-        *reinterpret_cast<float2*>(mid + (8 * k + g) * kRowBytes + place * 8) =
-            make_float2(fmaf(odd[2 * k], 0.0625f, even[2 * k]), fmaf(odd[2 * k + 1], 0.0625f, even[2 * k + 1]));
+    for (int i = 0; i < kSide; ++i) {
+      const int place = 8 * ((i0 + i) >> 1) + 2 * t + (i & 1);
+#pragma unroll
+      for (int k = 0; k < kR; ++k)
+        if (ROWS >= 8 || g < ROWS)
+          *reinterpret_cast<float2*>(mid + (8 * k + g) * kRowBytes + place * 8) =
+              make_float2(fmaf(odd[i][2 * k], 0.0625f, even[i][2 * k]),
+                          fmaf(odd[i][2 * k + 1], 0.0625f, even[i][2 * k + 1]));
+    }
   }
   // ----------------------------------------------------------------- softmax
   // This lane's keys: pair (i, t) = (lane / 4, lane % 4), the lane's place in a row likewise.
@@ -321,7 +330,7 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   for (int k = 0; k < kR; ++k) fix[k] = rescale;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    if (ROWS > 1 && r >= rows) break;
+    if (r % 4 == 0 && r >= rows) break;  // four rows at a time, for the distance between dependent steps
     uint8_t* at = mid + r * kRowBytes + place * 8;
     const float2 z = *reinterpret_cast<const float2*>(at);
     const int lim = __shfl_sync(0xffffffffu, limit, r);
@@ -451,7 +460,7 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Request& rq
 template <int HD, int ROWS>
 __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_attn_split_kernel(const AttnArgs a) {
   constexpr int kR = RowState<HD, ROWS>::kR;
-  constexpr int kS = kStages<HD>;
+  constexpr int kS = kStages<HD, ROWS>;
   constexpr int kThreads = kSplitWarps * 32;
   extern __shared__ __align__(128) uint8_t split_smem[];
   __shared__ uint64_t bars[kSplitWarps][kS];
