@@ -1,32 +1,14 @@
-// kv4_attn.cu — attention over the paged 4-bit KV cache (gsvk_kv4_attention).
+// kv4_attn.cu — attention over the paged 4-bit KV cache (gsvk_kv4_attention):
+// the kernel for requests with few new tokens (decoding, drafts) and the entry
+// points.  Long runs of new tokens are kv4_prompt.cu's.
 #include <algorithm>
 
 #include "gsvk_internal.hpp"
-#include "kv4.cuh"
-#include "tma.cuh"
+#include "kv4_attn.cuh"
 
 namespace gsvk {
 
 namespace {
-
-struct AttnArgs {
-  const uint8_t* pages;
-  size_t page_bytes;
-  int n_pages, shift, kv_heads;
-  const uint16_t* q;
-  size_t q_stride;
-  uint16_t* out;
-  size_t out_stride;
-  int heads, group, n_tokens, n_seq, max_blocks;
-  const int32_t* q_start;
-  const int32_t* kv_len;
-  const int32_t* prefix;
-  const int32_t* table;
-  float scale_log2;  // scale * log2(e)
-  int* tickets;      // of the items that several warps share
-  float* parts;      // their records
-  uint32_t* status;
-};
 
 // ------------------------------------------------------------ few query rows
 // Work.  An item is (request, kv head, block of up to ROWS query rows), a row
@@ -77,30 +59,10 @@ constexpr int kRowBytes = 32 * 8 + 32;
 template <int HD, int ROWS>
 constexpr int kWarpBytes = kStages<HD, ROWS> * kTileBytes<HD> + (ROWS * kRowBytes + 127) / 128 * 128;
 
-// One request's rows and the keys they see.
-struct Request {
-  int q0, n, len, prefix;
-};
-__device__ __forceinline__ Request request_of(const AttnArgs& a, int s) {
-  Request r;
-  r.q0 = a.q_start[s];
-  r.n = min(a.q_start[s + 1], a.n_tokens) - r.q0;
-  if (r.q0 < 0) r.n = 0;
-  r.len = a.kv_len[s];
-  r.prefix = a.prefix ? a.prefix[s] : 0;
-  return r;
-}
-// Keys that query row `row` of a request's kv head sees (64-bit on the way: lengths are the caller's).
-__device__ __forceinline__ int limit_of(const AttnArgs& a, const Request& q, int row) {
-  const int r = q.n == 1 || a.group == 1 ? (q.n == 1 ? 0 : row) : row / a.group;
-  const long long causal = static_cast<long long>(q.len) - q.n + r + 1;
-  const long long see = max(causal, static_cast<long long>(q.prefix));
-  const long long have = min(q.len, a.max_blocks << a.shift);
-  return static_cast<int>(max(0LL, min(see, have)));
-}
 template <int ROWS>
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, const Request& q) {
-  return q.n > 0 ? (q.n * a.group + ROWS - 1) / ROWS : 0;
+  const int rows = q.n * a.group;
+  return rows <= 0 || rows > a.most_rows ? 0 : (rows + ROWS - 1) / ROWS;  // more rows: kv4_prompt.cu's
 }
 // Keys that any row of a block sees.
 template <int ROWS>
@@ -171,12 +133,6 @@ __device__ __forceinline__ void mma_16816_first(float* d, uint32_t a0, uint32_t 
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // The state of ROWS query rows over the tiles seen so far.  As an MMA operand
 // lane (g, t) = (lane / 4, lane % 4) has row g (ROWS = 16: and row g + 8); its
 // part of the sums o is head_dim / 4 dimensions from t head_dim / 4 on (up to 8 rows: in two
@@ -286,7 +242,7 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
     }
 #pragma unroll
     for (int i = 0; i < kSide; ++i) {
-      const int place = 8 * ((i0 + i) >> 1) + 2 * t + (i & 1);
+      const int place = 8 * ((i0 + i) >> 1) + 2 * t + ((i0 + i) & 1);
 #pragma unroll
       for (int k = 0; k < kR; ++k)
         if (ROWS >= 8 || g < ROWS)
@@ -417,13 +373,6 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   }
 }
 
-// Where query row `row` of a request's kv head goes.
-__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, const Request& rq, int head, int row, int hd) {
-  const int r = rq.n == 1 ? 0 : row / a.group;
-  return a.out + static_cast<size_t>(rq.q0 + r) * a.out_stride +
-         static_cast<size_t>(head * a.group + row - r * a.group) * hd;
-}
-
 // Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.
 template <int HD, int ROWS>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int block, int first, int last,
@@ -471,6 +420,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
   uint8_t* ring = split_smem + warp * kWarpBytes<HD, ROWS>;
   uint8_t* mid = ring + kS * kTileBytes<HD>;
   const int warps = static_cast<int>(gridDim.x) * kSplitWarps;
+
+  griddep_launch_dependents();  // the kernel for longer requests may start beside this one
 
   // the line of units: each thread sums a run of requests
   const int per = (a.n_seq + kThreads - 1) / kThreads;
@@ -715,6 +666,9 @@ int launch_split(const AttnArgs& a, cudaStream_t st) {
   return check_launch("kv4_attn_split_kernel");
 }
 
+// Query rows of a request to a kv head from which on 128-row tiles are used.
+constexpr int kMostSplitRows = 64;
+
 // Tickets (zero between calls), then the records.
 size_t split_warps(size_t hd) {
   return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
@@ -731,7 +685,7 @@ extern "C" {
 size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads, size_t kv_heads,
                                     size_t head_dim) {
   if (n_seq == 0 || n_seq > 16384 || kv_heads == 0 || kv_heads > 1024 || heads % kv_heads ||
-      heads == 0 || heads > 65536 || n_tokens > 0x7fffffff ||
+      heads == 0 || heads > 65536 || n_tokens > 0x7fffffff / (heads / kv_heads) ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return 0;
   return tickets_bytes(head_dim) + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float);
@@ -786,15 +740,24 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + tickets_bytes(hd));
   a.status = device_status();
   cudaStream_t st = as_cuda(stream);
-  // as few MMA and softmax rows as the requests' tokens need
+  // Requests with more rows than this take the kernel with 128-row tiles.
   const size_t rows = g->max_q * a.group;
-  const auto run = [&](auto launch32, auto launch64, auto launch128) {
+  const bool prompts = rows > kMostSplitRows;
+  a.most_rows = prompts ? kMostSplitRows : 0x7fffffff;
+  // as few MMA and softmax rows as the requests' tokens need
+  const auto split = [&](auto launch32, auto launch64, auto launch128) {
     return hd == 32 ? launch32(a, st) : hd == 64 ? launch64(a, st) : launch128(a, st);
   };
-  if (rows <= 1) return run(launch_split<32, 1>, launch_split<64, 1>, launch_split<128, 1>);
-  if (rows <= 4) return run(launch_split<32, 4>, launch_split<64, 4>, launch_split<128, 4>);
-  if (rows <= 8) return run(launch_split<32, 8>, launch_split<64, 8>, launch_split<128, 8>);
-  return run(launch_split<32, 16>, launch_split<64, 16>, launch_split<128, 16>);
+  int rc;
+  if (rows <= 1)
+    rc = split(launch_split<32, 1>, launch_split<64, 1>, launch_split<128, 1>);
+  else if (rows <= 4)
+    rc = split(launch_split<32, 4>, launch_split<64, 4>, launch_split<128, 4>);
+  else if (rows <= 8)
+    rc = split(launch_split<32, 8>, launch_split<64, 8>, launch_split<128, 8>);
+  else
+    rc = split(launch_split<32, 16>, launch_split<64, 16>, launch_split<128, 16>);
+  return rc || !prompts ? rc : kv4_prompt_run(a, hd, st);
 }
 
 }  // extern "C"
