@@ -14,14 +14,24 @@
 // Mathematics.  With k_j = a_j c_j + b_j and v_j = s_j e_j + f_j (step, code,
 // low), c and e the codes,
 //   z_j = a_j (q.c_j) + b_j sum(q),          p_j = 2^(z_j - reference)
-//   out = (sum_j (p_j s_j) (e_j - 8) + sum_j p_j (f_j + 8 s_j)) / sum_j p_j,
-// so the tensor cores multiply codes, which are exact in fp16 (c as the
-// subnormal c 2^-24, one AND for two of them), q is not rounded, and the one
-// rounding to fp16 beside the result's is that of the weights p_j s_j, which meet
-// codes centred on zero: 2^-11 of the centred values' spread.
+// so the score MMAs multiply codes, which are exact in fp16 (c as the
+// subnormal c 2^-24, one AND for two of them), and q is not rounded.  The
+// values go in two ways:
+//   head_dim 32, 64: v_j as the sum of two fp16 numbers, side by side as
+//     2 head_dim columns of one operand (an MMA of 128 x 128 takes the 67 clocks that one of
+//     128 x 64 takes: measured), so the weights are p_j and need no
+//     parameters of the key;
+//   head_dim 128, where that would double the MMAs:
+//     sum_j p_j v_j = sum_j (p_j s_j) (e_j - 8) + sum_j p_j (f_j + 8 s_j).
+// Either way the one rounding to fp16 beside the result's is that of the
+// weights: 2^-11 of the values (centred ones for head_dim 128).
 // The reference is the row's maximum as of the last time that it grew by 2^8:
-// until then the weights (at most 2^10) stay in fp16's range and the sums in TMEM are
-// left alone.  Steps are divided by a power of two, the same for all rows.
+// until then the weights stay in fp16's range and the sums in TMEM are left
+// alone.  Values (steps) are divided by a power of two, the same for all rows.
+//
+// What bounds it: per 128 x 64 scores an SM's 16 exponentials a clock take 512
+// clocks, the MMAs 8 x 67 at head_dim 64, and the keys' parameters, which every
+// thread reads from shared memory (8 bytes a score, 128 bytes a clock), another 512.
 #include <algorithm>
 
 #include "gsvk_internal.hpp"
@@ -39,11 +49,16 @@ constexpr uint32_t kPTmemCols = 256;  // scores at 0 and 64, sums at 128
 
 // What the softmax needs of a tile's keys.
 struct alignas(16) TileParams {
-  float a[kPTile], b[kPTile], s[kPTile], f[kPTile];
-  float unit, rescale;  // the steps' unit, and the previous tile's over it
+  float a[kPTile], b[kPTile];
+  float s[kPTile], f[kPTile];  // head_dim 128
+  float unit, rescale;         // the values' unit, and the previous tile's over it
   uint32_t page_ok;
 };
 
+template <int HD>
+constexpr bool kPSplit = HD <= 64;  // values as two fp16 numbers
+template <int HD>
+constexpr int kPCols = kPSplit<HD> ? 2 * HD : HD;  // columns of the value operand and of the sums
 template <int HD>
 constexpr int kPRaw = HD == 128 ? 3 : 4;  // raw tiles in flight
 template <int HD>
@@ -53,16 +68,18 @@ constexpr int kPQBytes = kPRows * HD * 2;
 template <int HD>
 constexpr int kPOpBytes = kPTile * HD * 2;
 template <int HD>
+constexpr int kPValBytes = kPTile * kPCols<HD> * 2;
+template <int HD>
 constexpr int kPRawBytes = kPTile * (HD + 8);
 template <int HD>
-constexpr int kPSmem = 1024 + kPQBytes<HD> + (2 + kPValues<HD>)*kPOpBytes<HD> + kPRaw<HD> * kPRawBytes<HD> +
+constexpr int kPSmem = 1024 + kPQBytes<HD> + 2 * kPOpBytes<HD> + kPValues<HD> * kPValBytes<HD> + kPRaw<HD> * kPRawBytes<HD> +
                        2 * static_cast<int>(sizeof(TileParams));
 
-// 16-byte unit u of row r of an operand tile: rows of 64 values in the 128-byte swizzle, head_dim 128 as two
-// slabs of `rows` rows, head_dim 32 as 64-byte rows in the 64-byte swizzle.
-template <int HD>
+// 16-byte unit u of row r of an operand tile with COLS columns: rows of 64 values in the 128-byte swizzle, 128
+// columns as two slabs of `rows` rows, 32 as 64-byte rows in the 64-byte swizzle.
+template <int COLS>
 __device__ __forceinline__ uint32_t unit_at(int r, int u, int rows) {
-  if constexpr (HD == 32) return r * 64 + ((u ^ ((r >> 1) & 3)) << 4);
+  if constexpr (COLS == 32) return r * 64 + ((u ^ ((r >> 1) & 3)) << 4);
   return (u >> 3) * rows * 128 + r * 128 + (((u & 7) ^ (r & 7)) << 4);
 }
 // Operand descriptor; lbo: bytes between 64-column slabs of an operand that is contiguous along M or N.
@@ -116,6 +133,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// N consecutive words of shared memory, in as few loads as they allow (aligned to their size, at most 16 bytes).
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  }
+}
+
 __device__ __forceinline__ int prompt_blocks(const AttnArgs& a, int s) {
   const Request q = request_of(a, s);
   const int rows = q.n * a.group;
@@ -130,7 +162,7 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + kPQBytes<HD>;
   uint8_t* sV = sK + 2 * kPOpBytes<HD>;
-  uint8_t* sRaw = sV + kV * kPOpBytes<HD>;
+  uint8_t* sRaw = sV + kV * kPValBytes<HD>;
   TileParams* par = reinterpret_cast<TileParams*>(sRaw + kRaw * kPRawBytes<HD>);
   __shared__ uint64_t raw_full[kRaw], raw_free[kRaw], k_full[2], k_free[2], v_full[kV], v_free[kV];
   __shared__ uint64_t par_full[2], par_free[2], s_full[2], p_full[2], o_done, all_done;
@@ -274,12 +306,13 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
           z[j / 2] = pair(v.x, v.y);
         }
       }
-      float top = -INFINITY;
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < kPTile / 2; ++j) {
         const float2 v = unpair(z[j]);
-        top = fmaxf(top, fmaxf(v.x, v.y));
+        tops[j & 3] = fmaxf(fmaxf(tops[j & 3], v.x), v.y);
       }
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       unit = t.unit;
       if (i == 0) {
         ref = top;
@@ -296,7 +329,7 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
         pb2 = mul2(pb2, pair(keep, keep));
         const float by = keep * t.rescale;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
+        for (int c = 0; c < kPCols<HD>; c += 16) {
           uint32_t o[16];
           tmem_ld16(tmem + lanes + 128 + c, o);
           tmem_ld_wait();
@@ -310,16 +343,17 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
       const uint64_t nb = pair(-base, -base);
       uint32_t w[kPTile / 2];
 #pragma unroll
-      for (int j = 0; j < kPTile; j += 4) {
-        const ulonglong2 ts = *reinterpret_cast<const ulonglong2*>(t.s + j), tf = *reinterpret_cast<const ulonglong2*>(t.f + j);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float2 d = unpair(add2(z[j / 2 + k], nb));
-          const uint64_t p = pair(ex2(d.x), ex2(d.y));
-          l2 = add2(l2, p);
-          pb2 = fma2(p, k ? tf.y : tf.x, pb2);
-          const float2 x = unpair(mul2(p, k ? ts.y : ts.x));
-          w[j / 2 + k] = f2h2(x.x, x.y);
+      for (int j = 0; j < kPTile / 2; ++j) {
+        const float2 d = unpair(add2(z[j], nb));
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        const uint64_t p = pair(e.x, e.y);
+        l2 = add2(l2, p);
+        if constexpr (kPSplit<HD>) {
+          w[j] = f2h2(e.x, e.y);
+        } else {
+          pb2 = fma2(p, *reinterpret_cast<const uint64_t*>(t.f + 2 * j), pb2);
+          const float2 x = unpair(mul2(p, *reinterpret_cast<const uint64_t*>(t.s + 2 * j)));
+          w[j] = f2h2(x.x, x.y);
         }
       }
       tmem_st16(tmem + lanes + buf * kPTile, w);
@@ -343,6 +377,13 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
         tmem_ld16(tmem + lanes + 128 + c, o);
+        if constexpr (kPSplit<HD>) {
+          uint32_t second[16];
+          tmem_ld16(tmem + lanes + 128 + HD + c, second);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(second[k]));
+        }
         tmem_ld_wait();
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -362,7 +403,7 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsUnpack));
     const int me = tid - 128, key = me >> 1, half = me & 1;  // two threads to a key
     const int sub_bytes = kv4_head_bytes(sub_shift, HD), sub_mask = (1 << sub_shift) - 1;
-    float unit = 0.f;
+    float unit = 0.f, per_unit = 0.f;
     for (int i = 0; i < tiles; ++i) {
       const int rs = i % kRaw, buf = i & 1, vb = i % kV;
       const uint32_t ph = static_cast<uint32_t>(i >> 1) & 1u;
@@ -373,53 +414,51 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
       const uint32_t page_ok = raw_ok[rs];
       const uint8_t* sub = raw + (key >> sub_shift) * sub_bytes;
       const int at = key & sub_mask;
-      {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(sub + at * (HD / 2) + half * (HD / 4));
+      uint32_t words[HD / 16];  // this thread's half of a key's codes
+      load_words<HD / 16>(sub + at * (HD / 2) + half * (HD / 4), words);
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) {
-          const uint32_t x = src[u];
-          *reinterpret_cast<uint4*>(sK + buf * kPOpBytes<HD> + unit_at<HD>(key, half * (HD / 16) + u, kPTile)) =
-              make_uint4(x & 0x000f000fu, x >> 4 & 0x000f000fu, x >> 8 & 0x000f000fu, x >> 12 & 0x000f000fu);
-        }
+      for (int u = 0; u < HD / 16; ++u) {
+        const uint32_t x = words[u];
+        *reinterpret_cast<uint4*>(sK + buf * kPOpBytes<HD> + unit_at<HD>(key, half * (HD / 16) + u, kPTile)) =
+            make_uint4(x & 0x000f000fu, x >> 4 & 0x000f000fu, x >> 8 & 0x000f000fu, x >> 12 & 0x000f000fu);
       }
-      // the greatest step of the values that some row sees (each warp for itself)
-      uint32_t most = 0;
+      const uint32_t kp = *reinterpret_cast<const uint32_t*>(sub + kv4_k_par(sub_shift, HD) + at * 4);
+      const uint32_t vp = *reinterpret_cast<const uint32_t*>(sub + kv4_v_par(sub_shift, HD) + at * 4);
+      float vs = h2f(static_cast<uint16_t>(vp)), vf = h2f(static_cast<uint16_t>(vp >> 16));
+      const bool seen = i * kPTile + key < keys && (page_ok >> (key >> sub_shift) & 1u);
+      const bool number = fabsf(fmaf(15.f, vs, vf)) <= 3.0e38f;
+      if (!seen || !number) vs = vf = 0.f;  // whatever the page holds there
+      // What sets the unit: the greatest value (split) or step of the tile; each warp works it out for all 64 keys.
+      float most = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int j = lane + 32 * c;
-        const uint32_t h = *reinterpret_cast<const uint16_t*>(raw + (j >> sub_shift) * sub_bytes +
+        const uint32_t p = *reinterpret_cast<const uint32_t*>(raw + (j >> sub_shift) * sub_bytes +
                                                               kv4_v_par(sub_shift, HD) + (j & sub_mask) * 4);
-        if (i * kPTile + j < keys && (page_ok >> (j >> sub_shift) & 1u) && h < 0x7c00u) most = max(most, h);
+        const float st = h2f(static_cast<uint16_t>(p)), lo = h2f(static_cast<uint16_t>(p >> 16));
+        const float m = kPSplit<HD> ? fmaxf(fabsf(lo), fabsf(fmaf(15.f, st, lo))) : fabsf(st);
+        if (i * kPTile + j < keys && (page_ok >> (j >> sub_shift) & 1u) && fabsf(fmaf(15.f, st, lo)) <= 3.0e38f)
+          most = fmaxf(most, m);
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      // a unit holds until a step passes four times it
+      most = warp_max(most);
+      // a unit holds until something passes four times it
       float rescale = 1.f;
-      const float step = h2f(static_cast<uint16_t>(most));
-      if (step > 4.f * unit) {
-        const float next = __uint_as_float((__float_as_uint(step) & 0x7f800000u) + 0x00800000u);
+      if (most > 4.f * unit) {
+        const float next = __uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u);
         rescale = unit / next;
         unit = next;
+        per_unit = 1.f / next;  // a power of two: exact
       }
       if (half == 0) {
-        const uint32_t kp = *reinterpret_cast<const uint32_t*>(sub + kv4_k_par(sub_shift, HD) + at * 4);
-        const uint32_t vp = *reinterpret_cast<const uint32_t*>(sub + kv4_v_par(sub_shift, HD) + at * 4);
-        float ka = h2f(static_cast<uint16_t>(kp)) * (a.scale_log2 * 16777216.f);
-        float kb = h2f(static_cast<uint16_t>(kp >> 16)) * a.scale_log2;
-        const float vs = h2f(static_cast<uint16_t>(vp)), vf = fmaf(8.f, vs, h2f(static_cast<uint16_t>(vp >> 16)));
-        float ps = unit > 0.f ? vs / unit : 0.f, pf = vf;
-        if (i * kPTile + key >= keys || !(page_ok >> (key >> sub_shift) & 1u)) {
-          ka = kb = ps = pf = 0.f;  // nobody's: whatever the page holds there
-        } else if (!(fabsf(vf) <= 3.0e38f)) {
-          // values that are not numbers reach the rows that see them by their score, which a row that does not see the
-          // key replaces
-          ka = __int_as_float(0x7fffffff);
-          ps = pf = 0.f;
-        }
         TileParams& t = par[buf];
-        t.a[key] = ka;
-        t.b[key] = kb;
-        t.s[key] = ps;
-        t.f[key] = pf;
+        // Values that are not numbers reach the rows that see them by their score, which a row that does not see the
+        // key replaces.
+        t.a[key] = !seen ? 0.f : number ? h2f(static_cast<uint16_t>(kp)) * (a.scale_log2 * 16777216.f) : __int_as_float(0x7fffffff);
+        t.b[key] = !seen ? 0.f : h2f(static_cast<uint16_t>(kp >> 16)) * a.scale_log2;
+        if constexpr (!kPSplit<HD>) {
+          t.s[key] = vs * per_unit;
+          t.f[key] = fmaf(8.f, vs, vf);
+        }
         if (me == 0) {
           t.unit = unit;
           t.rescale = rescale;
@@ -434,23 +473,38 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
       }
       ok = mbar_wait(&v_free[vb], (static_cast<uint32_t>(i / kV) & 1u) ^ 1u, a.status);
       if (!__all_sync(0xffffffffu, ok)) break;
-      {
-        const uint32_t* src =
-            reinterpret_cast<const uint32_t*>(sub + kv4_v_codes(sub_shift, HD) + at * (HD / 2) + half * (HD / 4));
-        const __half2 bias = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1024 + 8
+      load_words<HD / 16>(sub + kv4_v_codes(sub_shift, HD) + at * (HD / 2) + half * (HD / 4), words);
+      uint8_t* val = sV + vb * kPValBytes<HD>;
+      const uint64_t s2 = pair(vs * per_unit, vs * per_unit), f2 = pair(vf * per_unit, vf * per_unit);
 #pragma unroll
-        for (int u = 0; u < HD / 16; ++u) {
-          const uint32_t x = src[u];
-          uint32_t y[4];
+      for (int u = 0; u < HD / 16; ++u) {
+        uint32_t y[4], y2[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            y[k] = (x >> (4 * k) & 0x000f000fu) | 0x64006400u;  // 1024 + code
-            const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&y[k]), bias);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t c = (words[u] >> (4 * k) & 0x000f000fu) | 0x64006400u;  // 1024 + code
+          if constexpr (kPSplit<HD>) {
+            // two codes as fp32: 2^23 + code, less 2^23
+            const uint64_t e = add2(pair(__uint_as_float((words[u] >> (4 * k) & 15u) | 0x4b000000u),
+                                         __uint_as_float((words[u] >> (4 * k + 16) & 15u) | 0x4b000000u)),
+                                    pair(-8388608.f, -8388608.f));
+            const uint64_t v = fma2(e, s2, f2);
+            const float2 x = unpair(v);
+            const __half2 h = __floats2half2_rn(x.x, x.y);
+            const float2 b = __half22float2(h);
+            const float2 r = unpair(add2(v, pair(-b.x, -b.y)));
+            y[k] = *reinterpret_cast<const uint32_t*>(&h);
+            y2[k] = f2h2(r.x, r.y);
+          } else {
+            const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c),
+                                      __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));  // code - 8
             y[k] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          *reinterpret_cast<uint4*>(sV + vb * kPOpBytes<HD> + unit_at<HD>(key, half * (HD / 16) + u, kPTile)) =
-              make_uint4(y[0], y[1], y[2], y[3]);
         }
+        const int unit_no = half * (HD / 16) + u;
+        *reinterpret_cast<uint4*>(val + unit_at<kPCols<HD>>(key, unit_no, kPTile)) = make_uint4(y[0], y[1], y[2], y[3]);
+        if constexpr (kPSplit<HD>)
+          *reinterpret_cast<uint4*>(val + unit_at<kPCols<HD>>(key, HD / 8 + unit_no, kPTile)) =
+              make_uint4(y2[0], y2[1], y2[2], y2[3]);
       }
       fence_proxy_async_shared();
       __syncwarp();
@@ -511,9 +565,9 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
       asm volatile("bar.sync 1, 160;" ::: "memory");
       tc_fence_after();
       if (lane == 0) {
-        constexpr uint32_t sw = HD == 32 ? 4 : 2, rowb = HD == 32 ? 64 : 128, sbo = 8 * rowb;
+        constexpr uint32_t sw = HD == 32 ? 4 : 2, sbo = HD == 32 ? 512 : 1024;  // value rows: 128 bytes
         constexpr uint32_t idesc_s = idesc_f16_f32(kPRows, kPTile);
-        constexpr uint32_t idesc_o = idesc_f16_f32(kPRows, HD) | 1u << 16;  // B contiguous along N
+        constexpr uint32_t idesc_o = idesc_f16_f32(kPRows, kPCols<HD>) | 1u << 16;  // B contiguous along N
         const uint32_t q = smem_u32(sQ), k = smem_u32(sK), v = smem_u32(sV);
         bool ok = true;
         for (int i = 0; i <= tiles && ok; ++i) {
@@ -539,7 +593,7 @@ __global__ void __launch_bounds__(kPThreads, 2) kv4_prompt_kernel(const AttnArgs
 #pragma unroll
             for (int j = 0; j < kPTile / 16; ++j)
               tc_mma_f16_ts(tmem + 128, tmem + buf * kPTile + j * 8,
-                            operand_desc(v + vb * kPOpBytes<HD> + j * 16 * rowb, kPTile * 128, sbo, sw), idesc_o,
+                            operand_desc(v + vb * kPValBytes<HD> + j * 16 * 128, kPTile * 128, 1024, 2), idesc_o,
                             (p | j) ? 1u : 0u);
             tc_commit(&v_free[vb]);
             tc_commit(&o_done);
