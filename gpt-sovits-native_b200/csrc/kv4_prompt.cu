@@ -16,16 +16,17 @@
 // and one fused product for two codes, and b as one more column of K against
 // sum(q), which is two columns of Q.  So no score is rounded below fp32
 // (K as one fp16 number would move each by 2^-12 |q||k|).
-// sum_j p_j v_j = sum_j p_j s_j (e_j - 8) + sum_j p_j (f_j + 8 s_j) likewise; at head_dim 32 and 64
-// the two parts of s (e - 8) lie side by side as 2 head_dim columns of the value
-// operand (an MMA of 128 x 128 takes the 67 clocks that one of 128 x 64 takes: measured),
-// at head_dim 128 the operand is e - 8 and s goes into the weights.  The last sum
-// stays in the softmax.  Either way the one rounding to fp16 beside the result's is that of
-// the weights: 2^-11 of values centred within 8 steps.
+// v_j goes in as two fp16 parts at head_dim 32 and 64, side by side as
+// 2 head_dim columns of the value operand (an MMA of 128 x 128 takes the 67
+// clocks that one of 128 x 64 takes: measured).  At head_dim 128 that would double the MMAs:
+//   sum_j p_j v_j = sum_j (p_j s_j) (e_j - 8) + sum_j p_j (f_j + 8 s_j)
+// there, with the codes e - 8 as the operand and the last sum in the softmax.
+// Either way the one rounding to fp16 beside the result's is that of the
+// weights: 2^-11 of the values (centred within 8 steps at head_dim 128).
 // p_j = 2^(z_j - reference); the reference is the row's maximum as of the last
 // time that it grew by 2^8: until then the weights stay in fp16's range and the
-// sums in TMEM are left alone.  K and s are divided by a power of two, that of K
-// by tile, that of s the same for all rows.
+// sums in TMEM are left alone.  K and V (s) are divided by a power of two, that
+// of K by tile, that of V the same for all rows.
 //
 // What bounds it, per 256 x 128 scores at head_dim 64: 2 x (9 + 8) MMAs of 67 clocks = 2,278, 32,768
 // exponentials at 16 a clock = 2,048, 5,400 warp instructions at 4 a clock.
@@ -56,8 +57,7 @@ constexpr int kPCols = kPSplit<HD> ? 2 * HD : HD;  // columns of the value opera
 // What the softmax needs of a tile's keys.
 template <int HD>
 struct alignas(16) TileParams {
-  float f[kPTile<HD>];
-  float s[kPSplit<HD> ? 4 : kPTile<HD>];  // head_dim 128
+  float s[kPSplit<HD> ? 4 : kPTile<HD>], f[kPSplit<HD> ? 4 : kPTile<HD>];  // head_dim 128
   float score;          // scores' unit: z = S * score
   float unit, rescale;  // the values' unit, and the previous tile's over it
   uint32_t page_ok;
@@ -161,9 +161,10 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// Eight codes w of a row less `less`, times s, as the sum of two fp16 numbers, in the order of the word's
-// nibbles: 0 4, 1 5, 2 6, 3 7.
-__device__ __forceinline__ void two_parts(uint32_t w, __half2 less, __half2 s, uint4* first, uint4* second) {
+// Eight codes w of a row, times s, as the sum of two fp16 numbers, in the order of the word's nibbles:
+// 0 4, 1 5, 2 6, 3 7.
+__device__ __forceinline__ void two_parts(uint32_t w, __half2 s, uint4* first, uint4* second) {
+  const __half2 less = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));
   uint32_t y[4], z[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -172,6 +173,23 @@ __device__ __forceinline__ void two_parts(uint32_t w, __half2 less, __half2 s, u
     const __half2 h = __hmul2(e, s), r = __hfma2(e, s, __hneg2(h));  // exact: 15 bits in all
     y[k] = *reinterpret_cast<const uint32_t*>(&h);
     z[k] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  *first = make_uint4(y[0], y[1], y[2], y[3]);
+  *second = make_uint4(z[0], z[1], z[2], z[3]);
+}
+// The same plus `low`.  The sum's rounding error is that of Knuth's two-sum, exact too.
+__device__ __forceinline__ void two_parts(uint32_t w, __half2 s, __half2 low, uint4* first, uint4* second) {
+  const __half2 less = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));
+  uint32_t y[4], z[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t c = (w >> (4 * k) & 0x000f000fu) | 0x64006400u;
+    const __half2 e = __hsub2(*reinterpret_cast<const __half2*>(&c), less);
+    const __half2 h = __hmul2(e, s), r = __hfma2(e, s, __hneg2(h));
+    const __half2 sum = __hadd2(h, low), b = __hsub2(sum, h);
+    const __half2 rest = __hadd2(__hadd2(__hsub2(h, __hsub2(sum, b)), __hsub2(low, b)), r);
+    y[k] = *reinterpret_cast<const uint32_t*>(&sum);
+    z[k] = *reinterpret_cast<const uint32_t*>(&rest);
   }
   *first = make_uint4(y[0], y[1], y[2], y[3]);
   *second = make_uint4(z[0], z[1], z[2], z[3]);
@@ -335,23 +353,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
           ok = false;
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        uint32_t r[kT];
-#pragma unroll
-        for (int c = 0; c < kT; c += 16) tmem_ld16(scores + c, r + c);
         const float score = t.score, rescale = t.rescale;
         const uint32_t page_ok = t.page_ok;
         unit = t.unit;
-        tmem_ld_wait();
-        if (i * kT + kT > least || page_ok != (1u << subs) - 1u) {
-          const int see = limit - i * kT;
+        // Two passes over the scores, 32 at a time: loops that stay small in the instruction caches, which three roles
+        // share.
+        const bool mask = i * kT + kT > least || page_ok != (1u << subs) - 1u;
+        const int see = limit - i * kT;
+        const auto load = [&](int c, uint32_t* r) {
+          tmem_ld16(scores + c, r);
+          tmem_ld16(scores + c + 16, r + 16);
+          tmem_ld_wait();
+          if (mask) {
 #pragma unroll
-          for (int j = 0; j < kT; ++j)
-            if (j >= see || !(page_ok >> (j >> sub_shift) & 1u)) r[j] = 0xff800000u;  // -infinity
-        }
+            for (int j = 0; j < 32; ++j)
+              if (c + j >= see || !(page_ok >> ((c + j) >> sub_shift) & 1u)) r[j] = 0xff800000u;  // -infinity
+          }
+        };
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < kT; c += 32) {
+          uint32_t r[32];
+          load(c, r);
 #pragma unroll
-        for (int j = 0; j < kT; j += 2)
-          tops[(j >> 1) & 3] = fmaxf(fmaxf(tops[(j >> 1) & 3], __uint_as_float(r[j])), __uint_as_float(r[j + 1]));
+          for (int j = 0; j < 32; j += 2)
+            tops[(j >> 1) & 3] = fmaxf(fmaxf(tops[(j >> 1) & 3], __uint_as_float(r[j])), __uint_as_float(r[j + 1]));
+        }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * score;
         if (i == 0) {
           ref = top;
@@ -376,21 +403,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         }
         const float base = ref == -INFINITY ? 0.f : ref;
         const uint64_t nb = pair(-base, -base), sc = pair(score, score);
+        uint64_t more = 0;  // a second sum: the distance between dependent additions
+#pragma unroll 1
+        for (int c = 0; c < kT; c += 32) {
+          uint32_t r[32];
+          load(c, r);
 #pragma unroll
-        for (int j = 0; j < kT / 2; ++j) {
-          const float2 d = unpair(fma2(pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sc, nb));
-          const float2 e = make_float2(ex2(d.x), ex2(d.y));
-          const uint64_t p = pair(e.x, e.y);
-          l2 = add2(l2, p);
-          pb2 = fma2(p, *reinterpret_cast<const uint64_t*>(t.f + 2 * j), pb2);
-          if constexpr (kPSplit<HD>) {
-            r[j] = f2h2(e.x, e.y);
-          } else {
-            const float2 x = unpair(mul2(p, *reinterpret_cast<const uint64_t*>(t.s + 2 * j)));
-            r[j] = f2h2(x.x, x.y);
+          for (int j = 0; j < 16; ++j) {
+            const float2 d = unpair(fma2(pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sc, nb));
+            const float2 e = make_float2(ex2(d.x), ex2(d.y));
+            const uint64_t p = pair(e.x, e.y);
+            if (j & 1) {
+              more = add2(more, p);
+            } else {
+              l2 = add2(l2, p);
+            }
+            if constexpr (kPSplit<HD>) {
+              r[j] = f2h2(e.x, e.y);
+            } else {
+              pb2 = fma2(p, *reinterpret_cast<const uint64_t*>(t.f + c + 2 * j), pb2);
+              const float2 x = unpair(mul2(p, *reinterpret_cast<const uint64_t*>(t.s + c + 2 * j)));
+              r[j] = f2h2(x.x, x.y);
+            }
           }
-          if ((j & 15) == 15) tmem_st16(scores + j - 15, r + j - 15);
+          tmem_st16(scores + c / 2, r);  // over scores that have been read
         }
+        l2 = add2(l2, more);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -436,7 +474,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
     // ----------------------------------------------------------------- unpack
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsUnpack));
     constexpr int kPer = 128 / kT;           // threads to a key
-    constexpr int kWords = HD / 8 / kPer;    // words of codes of a thread
+    constexpr int kWords = HD / 8 / kPer;    // words of codes of a thread, kStep at a time
+    constexpr int kStep = kWords >= 4 ? 4 : 2;
     const int me = tid - 256, key = me / kPer, part = me % kPer;
     const int sub_bytes = kv4_head_bytes(sub_shift, HD), sub_mask = (1 << sub_shift) - 1;
     float unit = 0.f, per_unit = 0.f;
@@ -452,9 +491,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       const int at = key & sub_mask;
       const uint32_t kp = *reinterpret_cast<const uint32_t*>(sub + kv4_k_par(sub_shift, HD) + at * 4);
       const uint32_t vp = *reinterpret_cast<const uint32_t*>(sub + kv4_v_par(sub_shift, HD) + at * 4);
-      uint32_t words[kWords], values[kWords];
-      load_words<kWords>(sub + at * (HD / 2) + part * (kWords * 4), words);
-      load_words<kWords>(sub + kv4_v_codes(sub_shift, HD) + at * (HD / 2) + part * (kWords * 4), values);
+      const uint8_t* key_codes = sub + at * (HD / 2) + part * (kWords * 4);
+      const uint8_t* value_codes = key_codes + kv4_v_codes(sub_shift, HD);
       float ks = h2f(static_cast<uint16_t>(kp)), kl = h2f(static_cast<uint16_t>(kp >> 16));
       float vs = h2f(static_cast<uint16_t>(vp)), vf = h2f(static_cast<uint16_t>(vp >> 16));
       // What lies past every row's limit or in a page that is not there counts as zero.  Keys or values that are
@@ -462,9 +500,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       const bool seen = i * kT + key < keys && (page_ok >> (key >> sub_shift) & 1u);
       const bool number = fabsf(ks) + fabsf(kl) + fabsf(vs) + fabsf(vf) <= 3.0e38f;
       if (!seen || !number) ks = kl = vs = vf = 0.f;
-      // the units: the greatest key (or 16 steps) and the greatest step of the tile
+      // the units: the greatest key and value (or 16 steps; for head_dim 128 the greatest step) of the tile
       {
-        const float mk = warp_max(fmaxf(fabsf(kl), 16.f * ks)), mv = warp_max(vs);
+        const float mk = warp_max(fmaxf(fabsf(kl), 16.f * ks)), mv = warp_max(kPSplit<HD> ? fmaxf(fabsf(vf), 16.f * vs) : vs);
         if (lane == 0) {
           s_most[buf][warp - 8] = make_float2(mk, mv);
           mbar_arrive(&most_full[buf]);
@@ -476,7 +514,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       const float most_k = fmaxf(fmaxf(m0.x, m0.z), fmaxf(m1.x, m1.z)), most_v = fmaxf(fmaxf(m0.y, m0.w), fmaxf(m1.y, m1.w));
       float per_key;
       const float key_unit = unit_above(most_k, &per_key);
-      float rescale = 1.f;  // a steps' unit holds until something passes four times it
+      float rescale = 1.f;  // the values' unit holds until something passes four times it
       if (most_v > 4.f * unit) {
         const float last = unit;
         unit = unit_above(most_v, &per_unit);
@@ -485,14 +523,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       uint8_t* keys_at = sK + buf * kPKeyBytes<HD>;
       {
         const __half2 s2 = __float2half2_rn(ks * per_key);
-        const __half2 less = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));
+#pragma unroll 1
+        for (int u = 0; u < kWords; u += kStep) {
+          uint32_t w[kStep];
+          load_words<kStep>(key_codes + 4 * u, w);
 #pragma unroll
-        for (int u = 0; u < kWords; ++u) {
-          uint4 first, second;
-          two_parts(words[u], less, s2, &first, &second);
-          const uint32_t to = unit_at<HD>(key, part * kWords + u, kT);
-          *reinterpret_cast<uint4*>(keys_at + to) = first;
-          *reinterpret_cast<uint4*>(keys_at + kPHalfBytes<HD> + to) = second;
+          for (int k = 0; k < kStep; ++k) {
+            uint4 first, second;
+            two_parts(w[k], s2, &first, &second);
+            const uint32_t to = unit_at<HD>(key, part * kWords + u + k, kT);
+            *reinterpret_cast<uint4*>(keys_at + to) = first;
+            *reinterpret_cast<uint4*>(keys_at + kPHalfBytes<HD> + to) = second;
+          }
         }
       }
       {
@@ -500,8 +542,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         if (part == 0) {
           const float low = seen && !number ? __int_as_float(0x7fffffff) : kl * per_key;
           put_two(keys_at + 2 * kPHalfBytes<HD>, key, low * 128.f, low * 0.0625f);
-          t.f[key] = fmaf(8.f, vs, vf);
-          if constexpr (!kPSplit<HD>) t.s[key] = vs * per_unit;
+          if constexpr (!kPSplit<HD>) {
+            t.s[key] = vs * per_unit;
+            t.f[key] = fmaf(8.f, vs, vf);
+          }
         }
         if (me == 0) {
           t.score = fmaxf(fabsf(a.scale_log2) * key_unit, 1e-30f);  // not 0, which a hidden score could not be scaled by
@@ -520,25 +564,30 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       if (!__all_sync(0xffffffffu, ok)) break;
       {
         uint8_t* dst = sV + buf * kPValBytes<HD>;
-        const __half2 s2 = __float2half2_rn(vs * per_unit);
-        const __half2 less = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1024 + 8
+        const __half2 s2 = __float2half2_rn(vs * per_unit), low2 = __float2half2_rn(vf * per_unit);
+#pragma unroll 1
+        for (int u = 0; u < kWords; u += kStep) {
+          uint32_t w[kStep];
+          load_words<kStep>(value_codes + 4 * u, w);
 #pragma unroll
-        for (int u = 0; u < kWords; ++u) {
-          const int to = part * kWords + u;
-          if constexpr (kPSplit<HD>) {
+          for (int k = 0; k < kStep; ++k) {
+            const int to = part * kWords + u + k;
             uint4 first, second;
-            two_parts(values[u], less, s2, &first, &second);
-            *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, to, kT)) = first;
-            *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, HD / 8 + to, kT)) = second;
-          } else {
-            uint32_t y[4];
+            if constexpr (kPSplit<HD>) {
+              two_parts(w[k], s2, low2, &first, &second);
+              *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, HD / 8 + to, kT)) = second;
+            } else {
+              uint32_t y[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t c = (values[u] >> (4 * k) & 0x000f000fu) | 0x64006400u;
-              const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c), less);
-              y[k] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t c = (w[k] >> (4 * j) & 0x000f000fu) | 0x64006400u;
+                const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c),
+                                          __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));  // code - 8
+                y[j] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              first = make_uint4(y[0], y[1], y[2], y[3]);
             }
-            *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, to, kT)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, to, kT)) = first;
           }
         }
       }
