@@ -11,13 +11,10 @@ namespace gsvk {
 namespace {
 
 // ------------------------------------------------------------ few query rows
-// Work.  An item is (request, kv head, block of up to ROWS query rows), a row
-// being one (new token, query head of the group); its unit of work is a tile
-// of 64 keys.  The units of all items lie on one line (request, head, block,
-// tile), which is cut into equal runs, one per warp of the grid, so ragged
-// lengths leave no warp idle and a single long request fills the GPU.  Every
-// CTA works the line out for itself from the lengths (a block-wide sum over
-// the requests).  An item cut between warps is joined by the warp that
+// Work.  The line of units (kv4_attn.cuh) in tiles of 64 keys is cut into one
+// run per warp of the grid, so ragged lengths leave no warp idle and a single
+// long request fills the GPU.  Every CTA works the line out for itself from
+// the lengths.  An item cut between warps is joined by the warp that
 // arrives last, in the order of the runs, so results do not depend on timing.
 //
 // Data.  A tile is one contiguous block per page and head; a lane per page
@@ -58,65 +55,6 @@ constexpr int kRecord = HD + 4;  // floats of a joined row: maximum, sum, (pad),
 constexpr int kRowBytes = 32 * 8 + 32;
 template <int HD, int ROWS>
 constexpr int kWarpBytes = kStages<HD, ROWS> * kTileBytes<HD> + (ROWS * kRowBytes + 127) / 128 * 128;
-
-template <int ROWS>
-__device__ __forceinline__ int blocks_of(const AttnArgs& a, const Request& q) {
-  const int rows = q.n * a.group;
-  return rows <= 0 || rows > a.most_rows ? 0 : (rows + ROWS - 1) / ROWS;  // more rows: kv4_prompt.cu's
-}
-// Keys that any row of a block sees.
-template <int ROWS>
-__device__ __forceinline__ int keys_of(const AttnArgs& a, const Request& q, int block) {
-  return limit_of(a, q, min((block + 1) * ROWS, q.n * a.group) - 1);
-}
-__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kTile - 1) / kTile); }
-// Units of one kv head of a request; *most keeps the longest item.
-template <int ROWS>
-__device__ __forceinline__ long long head_units(const AttnArgs& a, const Request& q, int* most) {
-  long long u = 0;
-  const int nb = blocks_of<ROWS>(a, q);
-#pragma unroll 1
-  for (int b = 0; b < nb; ++b) {
-    const int t = tiles_of(keys_of<ROWS>(a, q, b));
-    u += t;
-    *most = max(*most, t);
-  }
-  return u;
-}
-
-// A place on the line of units.
-template <int ROWS>
-struct Cursor {
-  Request req;
-  int seq, head, block, blocks, tile, tiles, keys;
-
-  __device__ __forceinline__ void set_block(const AttnArgs& a, int b) {
-    block = b;
-    keys = keys_of<ROWS>(a, req, b);
-    tiles = tiles_of(keys);
-  }
-  __device__ __forceinline__ void enter(const AttnArgs& a, int s) {
-    seq = s;
-    req = request_of(a, s);
-    blocks = blocks_of<ROWS>(a, req);
-  }
-  __device__ __forceinline__ void next_item(const AttnArgs& a) {
-    tile = 0;
-    if (++block == blocks) {
-      block = 0;
-      if (++head == a.kv_heads) {
-        head = 0;
-        do {
-          if (seq + 1 >= a.n_seq) return;  // the end of the line
-          enter(a, seq + 1);
-        } while (blocks == 0);
-      } else if (blocks == 1) {
-        return;
-      }
-    }
-    set_block(a, block);
-  }
-};
 
 __device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -413,9 +351,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
   constexpr int kThreads = kSplitWarps * 32;
   extern __shared__ __align__(128) uint8_t split_smem[];
   __shared__ uint64_t bars[kSplitWarps][kS];
-  __shared__ long long s_before[kThreads + 1];
-  __shared__ long long s_share;
-  __shared__ int s_most;
+  using L = Line<ROWS, kTile, false>;
+  __shared__ typename L::template Runs<kThreads> runs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* ring = split_smem + warp * kWarpBytes<HD, ROWS>;
   uint8_t* mid = ring + kS * kTileBytes<HD>;
@@ -423,95 +360,23 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
 
   griddep_launch_dependents();  // the kernel for longer requests may start beside this one
 
-  // the line of units: each thread sums a run of requests
-  const int per = (a.n_seq + kThreads - 1) / kThreads;
-  if (tid == 0) s_most = 0;
   if (lane < kS) mbar_init(&bars[warp][lane], 1);
   fence_barrier_init();
-  long long inc = 0;
-  {
-    int most = 0;
-    for (int s = tid * per; s < min((tid + 1) * per, a.n_seq); ++s)
-      inc += a.kv_heads * head_units<ROWS>(a, request_of(a, s), &most);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    __syncthreads();  // s_most is there
-    if (lane == 0) atomicMax(&s_most, most);
-    s_before[tid + 1] = inc;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) inc += s_before[32 * (w + 1)];
-    __syncthreads();
-    s_before[tid + 1] = inc;
-    if (tid == 0) s_before[0] = 0;
-    if (tid == kThreads - 1)
-      // a run: an equal share, and no less than lets kMaxPieces warps cover the longest item
-      s_share = max((inc + warps - 1) / warps, static_cast<long long>((s_most + kMaxPieces - 1) / kMaxPieces));
-    __syncthreads();
-  }
-  const long long total = s_before[kThreads];
+  L::template measure<kThreads>(a, runs, warps, kMaxPieces);
+  const long long total = runs.before[kThreads];
   const int me = static_cast<int>(blockIdx.x) * kSplitWarps + warp;
-  const long long u0 = me * s_share, u1 = min(total, u0 + s_share);
+  const long long u0 = me * runs.share, u1 = min(total, u0 + runs.share);
   if (u0 >= u1) return;
   // from here on units count from u0: a run has fewer than 2^31
-  const int share = static_cast<int>(s_share);
+  const int share = static_cast<int>(runs.share);
   const int run = static_cast<int>(u1 - u0);
-
-  // the request that holds unit u0, then the head, block and tile
-  Cursor<ROWS> at;
-  {
-    int lo = 0, hi = kThreads;  // the last run of requests that starts at or before u0
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (s_before[m] <= u0) {
-        lo = m;
-      } else {
-        hi = m;
-      }
-    }
-    long long left = u0 - s_before[lo];
-    int s = lo * per, most = 0;
-    long long u = 1;
-#pragma unroll 1
-    for (;; s += 32) {  // a lane to a request of the run
-      const long long mine = s + lane < a.n_seq ? head_units<ROWS>(a, request_of(a, s + lane), &most) : 0;
-      long long sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const unsigned found = __ballot_sync(0xffffffffu, left < sum * a.kv_heads);
-      if (found) {
-        const int i = __ffs(static_cast<int>(found)) - 1;
-        s += i;
-        u = __shfl_sync(0xffffffffu, mine, i);
-        left -= __shfl_sync(0xffffffffu, sum - mine, i) * a.kv_heads;
-        break;
-      }
-      left -= __shfl_sync(0xffffffffu, sum, 31) * a.kv_heads;
-      if (s + 32 >= a.n_seq) return;  // not reached: u0 lies on the line
-    }
-    // left < kv_heads units of a request
-    at.head = (u >> 31) == 0 && (left >> 31) == 0 ? static_cast<int>(left) / static_cast<int>(u) : static_cast<int>(left / u);
-    left -= at.head * u;
-    at.enter(a, s);
-    at.set_block(a, 0);
-    while (left >= at.tiles && at.block + 1 < at.blocks) {
-      left -= at.tiles;
-      at.set_block(a, at.block + 1);
-    }
-    at.tile = static_cast<int>(left);
-  }
+  typename L::Cursor at = L::template place<kThreads>(a, runs, u0);
   int item_start = -at.tile;  // the item's tile 0, counted from u0
 
   const int sub_shift = min(a.shift, 6), subs = kTile >> sub_shift;  // pages of a tile, or parts of one
   // The copies run kS tiles ahead of the sums; the page of the next copy is
   // read one tile earlier still, so that nothing waits for it.
-  Cursor<ROWS> ahead = at;
+  typename L::Cursor ahead = at;
   int to_load = run;
   int page = -1;
   unsigned ok_bits = 0;  // 8 bits for each stage: pages that are there
@@ -669,11 +534,15 @@ int launch_split(const AttnArgs& a, cudaStream_t st) {
 // Query rows of a request to a kv head from which on 128-row tiles are used.
 constexpr int kMostSplitRows = 64;
 
-// Tickets (zero between calls), then the records.
+// The workspace: tickets of both kernels (zero between calls), then their records.
 size_t split_warps(size_t hd) {
   return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
 }
 size_t tickets_bytes(size_t hd) { return (split_warps(hd) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
+// Offset of the records: after both kernels' tickets.
+size_t attention_parts(size_t hd) { return tickets_bytes(hd) + kv4_prompt_ticket_bytes(); }
+// Whether some request of n_tokens rows may have enough for the kernel for longer requests.
+bool may_be_long(size_t n_tokens, size_t group) { return n_tokens * group > kMostSplitRows; }
 
 }  // namespace
 }  // namespace gsvk
@@ -688,7 +557,8 @@ size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads,
       heads == 0 || heads > 65536 || n_tokens > 0x7fffffff / (heads / kv_heads) ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return 0;
-  return tickets_bytes(head_dim) + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float);
+  return attention_parts(head_dim) + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float) +
+         (may_be_long(n_tokens, heads / kv_heads) ? kv4_prompt_part_bytes(head_dim) : 0);
 }
 
 int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
@@ -737,12 +607,15 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   a.table = g->block_table;
   a.scale_log2 = g->scale * 1.4426950408889634f;
   a.tickets = static_cast<int*>(g->workspace);
-  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(g->workspace) + tickets_bytes(hd));
+  uint8_t* ws = static_cast<uint8_t*>(g->workspace);
+  a.long_tickets = reinterpret_cast<int*>(ws + tickets_bytes(hd));
+  a.parts = reinterpret_cast<float*>(ws + attention_parts(hd));
+  a.long_parts = reinterpret_cast<float*>(ws + attention_parts(hd) + split_warps(hd) * 2 * 16 * (hd + 4) * sizeof(float));
   a.status = device_status();
   cudaStream_t st = as_cuda(stream);
   // Requests with more rows than this take the kernel with 128-row tiles.
   const size_t rows = g->max_q * a.group;
-  const bool prompts = rows > kMostSplitRows;
+  const bool prompts = rows > kMostSplitRows && may_be_long(g->n_tokens, a.group);
   a.most_rows = prompts ? kMostSplitRows : 0x7fffffff;
   // as few MMA and softmax rows as the requests' tokens need
   const auto split = [&](auto launch32, auto launch64, auto launch128) {
