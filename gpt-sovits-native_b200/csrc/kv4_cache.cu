@@ -35,14 +35,45 @@ struct RowArgs {
   size_t page_bytes;
   int shift, heads;
   const int64_t* slots;
-  long long rows;  // tokens * heads
+  int tokens;
+  int units;     // 16-byte units of a token's row: heads * head_dim / 8
+  int per_block; // tokens of a CTA; where a token has more units than a CTA threads, gridDim.y CTAs share it
 };
-
-// 8 values of a row as fp32.
-__device__ __forceinline__ void load8(const uint16_t* p, float* f) {
-  unpack8(ld_stream_u4(p), f);
+// This thread's token and unit within its row; false past either's end.
+__device__ __forceinline__ bool place_of(const RowArgs& a, int* t, int* u) {
+  const int k = static_cast<int>(threadIdx.x) / a.units;  // 0 where a token fills the CTA
+  *t = static_cast<int>(blockIdx.x) * a.per_block + k;
+  *u = static_cast<int>(threadIdx.x) - k * a.units + static_cast<int>(blockIdx.y) * kRowThreads;
+  return k < a.per_block && *t < a.tokens && *u < a.units;
 }
-__device__ __forceinline__ void load8(const float* p, float* f) {
+
+// 8 values of a row as fp32, and the extremes of the row, which is spread over L lanes.  A NaN makes both NaN.
+template <int L>
+__device__ __forceinline__ void load8(const uint16_t* p, float* f, float* lo, float* hi) {
+  const uint4 v = ld_stream_u4(p);
+  unpack8(v, f);
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const __half2 least = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+  const __half2 most = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  // the least value and the greatest, negated: one shuffle for both
+  __half2 m = __hmin2_nan(__lows2half2(least, __hneg2(most)), __highs2half2(least, __hneg2(most)));
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) m = __hmin2_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  *lo = __low2float(m);
+  *hi = -__high2float(m);
+}
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float m;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+template <int L>
+__device__ __forceinline__ void load8(const float* p, float* f, float* lo, float* hi) {
   const uint4 a = ld_stream_u4(p), b = ld_stream_u4(p + 4);
   f[0] = __uint_as_float(a.x);
   f[1] = __uint_as_float(a.y);
@@ -52,41 +83,62 @@ __device__ __forceinline__ void load8(const float* p, float* f) {
   f[5] = __uint_as_float(b.y);
   f[6] = __uint_as_float(b.z);
   f[7] = __uint_as_float(b.w);
-}
-
-// Codes of 8 of a row's values (spread over L lanes) and its parameters.
-template <int L>
-__device__ __forceinline__ uint32_t quantise8(const float* x, uint32_t* par) {
-  float lo = x[0], hi = x[0];
-  bool bad = false;
+  float least = f[0], most = f[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad |= !(fabsf(x[i]) < 65520.f);  // NaN, infinite, or rounds to an fp16 infinity
+  for (int i = 1; i < 8; ++i) {
+    least = min_nan(least, f[i]);
+    most = max_nan(most, f[i]);
   }
 #pragma unroll
   for (int o = 1; o < L; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o) != 0;
+    least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, o));
+    most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
   }
+  *lo = least;
+  *hi = most;
+}
+
+// Codes of 8 of a row's values and its parameters.  HALF: fp16 values, of which none is below low.
+template <bool HALF>
+__device__ __forceinline__ uint32_t quantise8(const float* x, float lo, float hi, uint32_t* par) {
   const uint16_t low16 = f2h(lo), step16 = f2h(__fdiv_rn(hi - lo, 15.f));
   const float low = h2f(low16), step = h2f(step16);
-  uint32_t w = 0;
-  if (step > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fdiv_rn(x[i] - low, step));
-      w |= static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) << (4 * i);
-    }
-  }
   *par = step16 | static_cast<uint32_t>(low16) << 16;
-  if (bad) {
-    w = 0;
-    *par = 0x7fff7fffu;  // NaN, NaN
+  if (!(fmaxf(-lo, hi) < 65520.f) || lo != lo) {  // infinite, rounds to an fp16 infinity, or NaN
+    *par = 0x7fff7fffu;                            // NaN, NaN
+    return 0;
   }
-  return w;
+  if (!(step > 0.f)) return 0;
+  // (x - low) * (1 / step) is within 6e-6 of the quotient (where that is below 16: the others are clamped either way);
+  // further than 1e-5 from a tie it rounds like the quotient, else the division itself is made.  A sum with 1.5 2^23 is
+  // rounded to an integer, to even, with the code in its low bits.
+  constexpr float kRound = 12582912.f;
+  float per_step;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per_step) : "f"(step));
+  const uint64_t minus_low = pair(-low, -low), per2 = pair(per_step, per_step);
+  const uint64_t up = pair(kRound, kRound), down = pair(-kRound, -kRound), minus = pair(-1.f, -1.f);
+  float c[8], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float2 q = unpair(mul2(add2(pair(x[i], x[i + 1]), minus_low), per2));
+    if (!HALF) q = make_float2(fmaxf(q.x, 0.f), fmaxf(q.y, 0.f));
+    const uint64_t q2 = pair(fminf(q.x, 15.f), fminf(q.y, 15.f)), c2 = add2(q2, up);
+    const float2 off = unpair(fma2(add2(c2, down), minus, q2)), r = unpair(c2);
+    c[i] = r.x;
+    c[i + 1] = r.y;
+    far = fmaxf(fmaxf(far, fabsf(off.x)), fabsf(off.y));
+  }
+  if (!(far < 0.49999f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(__fdiv_rn(x[i] - low, step), 0.f), 15.f) + kRound;
+  }
+  uint32_t w = 0, bits = 0;  // sums of the bits, less those of the eight 1.5 2^23
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w += __float_as_uint(c[i]) << (4 * i);
+    bits += 0x4b400000u << (4 * i);
+  }
+  return w - bits;
 }
 
 template <int HD, typename T>
@@ -94,20 +146,18 @@ __global__ void __launch_bounds__(kRowThreads)
     kv4_append_kernel(const RowArgs a, const T* __restrict__ k, size_t k_stride,
                       const T* __restrict__ v, size_t v_stride) {
   constexpr int L = HD / 8;
-  const long long row = (static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x) / L;
-  const int part = threadIdx.x % L;
-  // a warp's lanes all shuffle: those past the end repeat the last row and write nothing
-  const long long r = min(row, a.rows - 1);
-  const long long t = r / a.heads;
-  const int h = static_cast<int>(r - t * a.heads);
-  float xk[8], xv[8];
-  load8(k + t * k_stride + static_cast<size_t>(h) * HD + part * 8, xk);
-  load8(v + t * v_stride + static_cast<size_t>(h) * HD + part * 8, xv);
+  int t, u;
+  const bool there = place_of(a, &t, &u);
+  if (!there) t = u = 0;  // all lanes shuffle: these repeat the first row and write nothing
+  const int h = u / L, part = u % L;
+  float xk[8], xv[8], lo_k, hi_k, lo_v, hi_v;
+  load8<L>(k + t * k_stride + u * 8, xk, &lo_k, &hi_k);
+  load8<L>(v + t * v_stride + u * 8, xv, &lo_v, &hi_v);
   const int64_t slot = a.slots[t];
   uint32_t pk, pv;
-  const uint32_t wk = quantise8<L>(xk, &pk);
-  const uint32_t wv = quantise8<L>(xv, &pv);
-  if (row >= a.rows || slot < 0 || slot >= a.n_slots) return;
+  const uint32_t wk = quantise8<sizeof(T) == 2>(xk, lo_k, hi_k, &pk);
+  const uint32_t wv = quantise8<sizeof(T) == 2>(xv, lo_v, hi_v, &pv);
+  if (!there || slot < 0 || slot >= a.n_slots) return;
   const int at = static_cast<int>(slot & ((1 << a.shift) - 1));
   uint8_t* b = a.pages + static_cast<size_t>(slot >> a.shift) * a.page_bytes +
                static_cast<size_t>(h) * kv4_head_bytes(a.shift, HD);
@@ -119,20 +169,21 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-// The top level may lie above fp16's range (a step rounded up): held at its
-// greatest value.  NaN passes.
-__device__ __forceinline__ float in_range(float x) {
-  return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x;
-}
-// 8 codes -> fp16 values, rounded once.
+// 8 codes -> fp16 values: step * code + low as one fused fp16 operation, rounded once.  The top level may
+// lie above fp16's range (a step rounded up): held at its greatest value.  NaN passes.
 __device__ __forceinline__ uint4 values8(uint32_t w, uint32_t par) {
-  const float step = h2f(static_cast<uint16_t>(par)), low = h2f(static_cast<uint16_t>(par >> 16));
-  uint32_t o[4];
+  const __half2 p = *reinterpret_cast<const __half2*>(&par);
+  const __half2 step = __low2half2(p), low = __high2half2(p);
+  const __half2 top = __float2half2_rn(65504.f), bias = __float2half2_rn(1024.f);
+  uint32_t y[4];  // values k and k + 4
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    o[i] = f2h2(in_range(fmaf(step, static_cast<float>((w >> (8 * i)) & 15u), low)),
-                in_range(fmaf(step, static_cast<float>((w >> (8 * i + 4)) & 15u), low)));
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t c = (w >> (4 * k) & 0x000f000fu) | 0x64006400u;  // 1024 + code
+    const __half2 v = __hmin2_nan(__hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), bias), step, low), top);
+    y[k] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                    __byte_perm(y[2], y[3], 0x7632));
 }
 
 template <int HD>
@@ -140,11 +191,9 @@ __global__ void __launch_bounds__(kRowThreads)
     kv4_read_kernel(const RowArgs a, uint16_t* __restrict__ k, size_t k_stride,
                     uint16_t* __restrict__ v, size_t v_stride) {
   constexpr int L = HD / 8;
-  const long long r = (static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x) / L;
-  const int part = threadIdx.x % L;
-  if (r >= a.rows) return;
-  const long long t = r / a.heads;
-  const int h = static_cast<int>(r - t * a.heads);
+  int t, u;
+  if (!place_of(a, &t, &u)) return;
+  const int h = u / L, part = u % L;
   const int64_t slot = a.slots[t];
   uint4 yk = make_uint4(0, 0, 0, 0), yv = yk;
   if (slot >= 0 && slot < a.n_slots) {
@@ -157,33 +206,32 @@ __global__ void __launch_bounds__(kRowThreads)
     yk = values8(wk, *reinterpret_cast<const uint32_t*>(b + kv4_k_par(a.shift, HD) + at * 4));
     yv = values8(wv, *reinterpret_cast<const uint32_t*>(b + kv4_v_par(a.shift, HD) + at * 4));
   }
-  if (k) *reinterpret_cast<uint4*>(k + t * k_stride + static_cast<size_t>(h) * HD + part * 8) = yk;
-  if (v) *reinterpret_cast<uint4*>(v + t * v_stride + static_cast<size_t>(h) * HD + part * 8) = yv;
+  if (k) *reinterpret_cast<uint4*>(k + t * k_stride + u * 8) = yk;
+  if (v) *reinterpret_cast<uint4*>(v + t * v_stride + u * 8) = yv;
 }
 
-// Checks and fills what append and read share; *blocks receives the grid.
+// Checks and fills what append and read share; *grid receives the launch's.
 int row_args(const gsvk_kv4_cache* c, const int64_t* slots, size_t n_tokens, const char* who,
-             RowArgs* a, unsigned* blocks) {
+             RowArgs* a, dim3* grid) {
   if (int rc = kv4_check(c, who)) return rc;
   if (!slots && n_tokens) return fail(GSVK_ERR_INVALID, "%s: null slots", who);
-  const size_t lanes = static_cast<size_t>(c->head_dim) / 8;
-  if (n_tokens > 0x7fffffff ||
-      n_tokens * c->kv_heads * lanes > static_cast<size_t>(0x7fffffff) * kRowThreads)
-    return fail(GSVK_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (n_tokens > 0x7fffffff) return fail(GSVK_ERR_UNSUPPORTED, "%s: too many tokens", who);
   a->pages = c->pages;
   a->shift = kv4_page_shift(c->page_size);
   a->n_slots = static_cast<long long>(c->n_pages) << a->shift;
   a->page_bytes = gsvk_kv4_page_bytes(c->page_size, c->kv_heads, c->head_dim);
   a->heads = c->kv_heads;
   a->slots = slots;
-  a->rows = static_cast<long long>(n_tokens) * c->kv_heads;
-  *blocks = ceil_div(static_cast<size_t>(a->rows) * lanes, kRowThreads);
+  a->tokens = static_cast<int>(n_tokens);
+  a->units = c->kv_heads * (c->head_dim / 8);
+  a->per_block = std::max(1, kRowThreads / a->units);
+  *grid = dim3(ceil_div(n_tokens, a->per_block), ceil_div(a->units, kRowThreads));
   return GSVK_OK;
 }
 
 template <typename T>
 int append_run(const RowArgs& a, int hd, const void* k, size_t ks, const void* v, size_t vs,
-               unsigned blocks, cudaStream_t st) {
+               dim3 blocks, cudaStream_t st) {
   const T* kt = static_cast<const T*>(k);
   const T* vt = static_cast<const T*>(v);
   if (hd == 32) kv4_append_kernel<32><<<blocks, kRowThreads, 0, st>>>(a, kt, ks, vt, vs);
@@ -211,7 +259,7 @@ int gsvk_kv4_append(const gsvk_kv4_cache* c, const void* k, size_t k_stride, con
                     size_t v_stride, int is_f32, const int64_t* slots, size_t n_tokens,
                     gsvk_stream_t stream) {
   RowArgs a;
-  unsigned blocks = 0;
+  dim3 blocks;
   if (int rc = row_args(c, slots, n_tokens, "kv4_append", &a, &blocks)) return rc;
   if (n_tokens == 0) return GSVK_OK;
   if (!k || !v) return fail(GSVK_ERR_INVALID, "kv4_append: null rows");
@@ -228,7 +276,7 @@ int gsvk_kv4_append(const gsvk_kv4_cache* c, const void* k, size_t k_stride, con
 int gsvk_kv4_read(const gsvk_kv4_cache* c, const int64_t* slots, size_t n_tokens, uint16_t* k,
                   size_t k_stride, uint16_t* v, size_t v_stride, gsvk_stream_t stream) {
   RowArgs a;
-  unsigned blocks = 0;
+  dim3 blocks;
   if (int rc = row_args(c, slots, n_tokens, "kv4_read", &a, &blocks)) return rc;
   if (n_tokens == 0) return GSVK_OK;
   if (!k && !v) return fail(GSVK_ERR_INVALID, "kv4_read: no output");
