@@ -8,9 +8,9 @@
 // therefore repeats the scan for itself (16 KB of lengths from L2 at 4096
 // requests) instead of waiting for another CTA's, keeps both sums in shared
 // memory, and takes a contiguous share of the rows and of the granted pages,
-// each located by binary search.  The state that may alias an input (kv_len,
-// free_left) is written by the CTA that draws the last ticket, when every
-// other one has read it.
+// each located by binary search.  Where a result is an input's own buffer (a
+// step in place), the CTA that draws the last ticket writes the results, when
+// every other one has read the inputs; else the first CTA does, without a ticket.
 #include <algorithm>
 
 #include "gsvk_internal.hpp"
@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr size_t kPlanMaxSeq = 16384;
-constexpr int kPlanRowsPerCta = 4096;  // rows one CTA maps before another is launched
+constexpr int kPlanRowsPerCta = 2048;  // rows one CTA maps before another is launched
 
 struct PlanArgs {
   int n_seq, max_blocks, n_pages, page_shift;
@@ -38,6 +38,7 @@ struct PlanArgs {
   int32_t* free_left;
   int32_t* refused;
   int32_t* ticket;
+  int in_place;  // kv_len or free_left is an input too
 };
 
 __device__ __forceinline__ long long warp_incl_scan(long long v, int lane) {
@@ -48,17 +49,25 @@ __device__ __forceinline__ long long warp_incl_scan(long long v, int lane) {
   }
   return v;
 }
-// Exclusive block-wide prefix of v (kPlanThreads threads); *total receives the sum.
-__device__ long long block_excl_scan(long long v, long long* sh, long long* total) {
+// Exclusive block-wide prefixes of N values (kPlanThreads threads); total receives the sums.
+template <int N>
+__device__ __forceinline__ void block_excl_scan(long long* v, long long (*sh)[32], long long* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long inc = warp_incl_scan(v, lane);
+  long long inc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) inc[k] = warp_incl_scan(v[k], lane);
   __syncthreads();  // sh is free again
-  if (lane == 31) sh[warp] = inc;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (lane == 31) sh[k][warp] = inc[k];
   __syncthreads();
-  const long long w = warp_incl_scan(sh[lane], lane);  // 32 warps: every warp scans their sums
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  return inc - v + (warp ? before : 0);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long long w = warp_incl_scan(sh[k][lane], lane);  // 32 warps: every warp scans their sums
+    total[k] = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    v[k] = inc[k] - v[k] + (warp ? before : 0);
+  }
 }
 
 // The last i in [0, n) with start[i] <= x (start ascending, start[0] = 0); of
@@ -99,51 +108,54 @@ __device__ __forceinline__ Need need_of(const PlanArgs& a, int i) {
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* s_row = plan_smem;             // [n_seq + 1] first row (clamped to max_tokens + 1)
-  int32_t* s_page = plan_smem + a.n_seq + 1;  // [n_seq + 1] pages before; bitwise not of it: refused
-  __shared__ long long sh[32];
-  __shared__ int s_last, s_refused;
+  int32_t* s_page = plan_smem + a.n_seq + 1;  // [n_seq] pages before; bitwise not of it: refused
+  __shared__ long long sh[2][32];
+  __shared__ int s_last, s_refused, s_taken;
   const int tid = threadIdx.x;
   const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
   const int free_count = min(max(*a.free_count, 0), a.n_pages);
-  if (tid == 0) s_refused = 0;
+  if (tid == 0) s_refused = s_taken = 0;
 
-  // rows first: a request's rows decide whether it is valid, hence its pages
-  long long rows = 0;
-  for (int i = i0; i < i1; ++i) rows += need_of(a, i).rows;
-  long long total_rows;
-  const long long row0 = block_excl_scan(rows, sh, &total_rows);
-  const long long cap = a.max_tokens;
-  long long pages = 0, r = row0;
+  long long before[2] = {0, 0}, total[2];  // rows, pages
   for (int i = i0; i < i1; ++i) {
     const Need q = need_of(a, i);
-    r += q.rows;
-    if (r <= cap) pages += q.pages;
+    before[0] += q.rows;
+    before[1] += q.pages;
   }
-  long long total_pages;
-  long long page0 = block_excl_scan(pages, sh, &total_pages);
-  r = row0;
-  long long granted_pages = 0;
-  int refused = 0;
+  block_excl_scan<2>(before, sh, total);
+  const long long cap = a.max_tokens, total_rows = total[0];
+  long long row = before[0], page = before[1];
+  if (total_rows > cap) {  // those that end past the last row need no pages: their sum again, without them
+    long long r = row, pages = 0;
+    for (int i = i0; i < i1; ++i) {
+      const Need q = need_of(a, i);
+      r += q.rows;
+      if (r <= cap) pages += q.pages;
+    }
+    block_excl_scan<1>(&pages, sh, total);
+    page = pages;
+  }
+  int refused = 0, taken = 0;
   for (int i = i0; i < i1; ++i) {
     const Need q = need_of(a, i);
-    s_row[i] = static_cast<int>(min(r, cap + 1));
-    r += q.rows;
-    const int need = (r <= cap) ? q.pages : 0;
-    const bool ok = q.valid && r <= cap && (need == 0 || page0 + need <= free_count);
-    const int before = static_cast<int>(min(page0, static_cast<long long>(free_count)));
-    s_page[i] = ok ? before : ~before;
-    if (ok) granted_pages += need;
+    s_row[i] = static_cast<int>(min(row, cap + 1));
+    row += q.rows;
+    const int need = row <= cap ? q.pages : 0;
+    const bool ok = q.valid && row <= cap && (need == 0 || page + need <= free_count);
+    const int first = static_cast<int>(min(page, static_cast<long long>(free_count)));
+    s_page[i] = ok ? first : ~first;
+    page += need;
     if (!ok) ++refused;
-    page0 += need;
+    if (ok && need) taken = static_cast<int>(page);  // granted ones are those before the first shortage
   }
-  if (refused) atomicAdd(&s_refused, refused);
-  long long taken;
-  block_excl_scan(granted_pages, sh, &taken);
-  if (tid == 0) {
-    s_row[a.n_seq] = static_cast<int>(min(total_rows, cap + 1));
-    s_page[a.n_seq] = static_cast<int>(taken);
+  refused = __reduce_add_sync(0xffffffffu, refused);
+  taken = __reduce_max_sync(0xffffffffu, taken);
+  if ((tid & 31) == 0) {  // s_refused and s_taken were set before the sums' barriers
+    if (refused) atomicAdd(&s_refused, refused);
+    atomicMax(&s_taken, taken);
   }
+  if (tid == 0) s_row[a.n_seq] = static_cast<int>(min(total_rows, cap + 1));
   __syncthreads();
 
   const int live_rows = static_cast<int>(min(total_rows, cap));
@@ -182,7 +194,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
           a.free_pages[free_count - 1 - (before + b - have)];
   }
 
-  if (gridDim.x > 1) {
+  if (!a.in_place) {
+    if (blockIdx.x != 0) return;
+  } else if (gridDim.x > 1) {
     __syncthreads();  // this CTA has read its lengths and the free count
     if (tid == 0) {
       __threadfence();
@@ -200,9 +214,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
   }
   if (tid == 0) {
     a.q_start[a.n_seq] = s_row[a.n_seq];
-    *a.free_left = free_count - s_page[a.n_seq];
+    *a.free_left = free_count - s_taken;
     *a.refused = s_refused;
-    if (gridDim.x > 1) *a.ticket = 0;
+    if (a.in_place && gridDim.x > 1) *a.ticket = 0;
   }
 }
 
@@ -215,7 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads)
                       int32_t* __restrict__ table, int32_t* __restrict__ free_pages,
                       int32_t* __restrict__ free_count) {
   extern __shared__ int32_t rel_smem[];  // [n_seq] pages returned, then their first place
-  __shared__ long long sh[32];
+  __shared__ long long sh[1][32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int mask = (1 << page_shift) - 1;
   const int count = min(max(*free_count, 0), n_pages);
@@ -239,7 +253,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   const int i0 = min(tid * per, n_seq), i1 = min(i0 + per, n_seq);
   long long mine = 0, total;
   for (int i = i0; i < i1; ++i) mine += rel_smem[i];
-  long long at = count + block_excl_scan(mine, sh, &total);
+  block_excl_scan<1>(&mine, sh, &total);
+  long long at = count + mine;
   for (int i = i0; i < i1; ++i) {
     const int found = rel_smem[i];
     rel_smem[i] = static_cast<int>(min(at, static_cast<long long>(n_pages)));
@@ -286,7 +301,8 @@ int gsvk_kv_plan(const gsvk_kv_plan_args* g, gsvk_stream_t stream) {
   PlanArgs a{static_cast<int>(g->n_seq), static_cast<int>(g->max_blocks),
              static_cast<int>(g->n_pages), shift, static_cast<long long>(g->max_tokens),
              g->ctx_len, g->new_len, g->block_table, g->free_pages, g->free_count, g->q_start,
-             g->kv_len, g->slots, g->free_left, g->refused, g->workspace};
+             g->kv_len, g->slots, g->free_left, g->refused, g->workspace,
+             g->kv_len == g->ctx_len || g->kv_len == g->new_len || g->free_left == g->free_count};
   const size_t smem = 2 * (g->n_seq + 1) * sizeof(int32_t);
   if (smem > 48 * 1024)
     if (int rc = check_cuda(cudaFuncSetAttribute(kv_plan_kernel,
