@@ -11,31 +11,115 @@ namespace gsvk {
 namespace {
 
 // ------------------------------------------------------------ row quantiser
+// Memory bounds it (3 bytes a value in fp16): a row's values are read once in
+// 16-byte vectors, kept in registers between the maximum and the codes (kept in
+// cache for rows longer than THREADS lanes hold), and leave 8 codes at a time.
+// Short rows take a warp each, long ones a CTA.
 __device__ __forceinline__ float as_f32(uint16_t v) { return h2f(v); }
 __device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ void load8(const uint16_t* p, float* f) { unpack8(ld_stream_u4(p), f); }
+__device__ __forceinline__ void load8(const float* p, float* f) {
+  const uint4 a = ld_stream_u4(p), b = ld_stream_u4(p + 4);
+  const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
+}
 
-// One warp per row: the maximum, then the codes (the row is in L1 by then).
-template <typename T>
-__global__ void __launch_bounds__(256)
-    quantize_rows_kernel(const T* __restrict__ x, size_t ldx, long long rows, int n,
-                         int8_t* __restrict__ q, size_t ldq, float* __restrict__ scale) {
-  const long long r = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (r >= rows) return;
-  const T* xr = x + r * ldx;
-  float top = 0.f;
-  bool bad = false;
-  for (int i = lane; i < n; i += 32) {
-    const float v = fabsf(as_f32(xr[i]));
-    bad |= !(v <= 3.402823466e38f);
-    top = fmaxf(top, v);
+// 8 codes of a row with scale s > 0.  x * (1 / s) is within 1e-4 of the quotient (below 128): further than that from a tie
+// it rounds like the quotient, else the division itself is made.  A sum with 1.5 2^23 is rounded to an
+// integer, to even, with the code as its low byte.
+__device__ __forceinline__ uint2 codes8(const float* x, float s, float per_s) {
+  constexpr float kRound = 12582912.f;
+  float c[8], far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = x[i] * per_s;
+    c[i] = q + kRound;
+    far = fmaxf(far, fabsf(q - (c[i] - kRound)));
   }
-  top = warp_max(top);
-  bad = __any_sync(0xffffffffu, bad);
-  const float s = bad ? __int_as_float(0x7fffffff) : __fdiv_rn(top, 127.f);
-  for (int i = lane; i < n; i += 32)
-    q[r * ldq + i] = s > 0.f ? static_cast<int8_t>(rintf(__fdiv_rn(as_f32(xr[i]), s))) : 0;
-  if (lane == 0) scale[r] = s;
+  if (!(far < 0.4998f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __fdiv_rn(x[i], s) + kRound;
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(__float_as_uint(c[4 * i]), __float_as_uint(c[4 * i + 1]), 0x0040),
+                       __byte_perm(__float_as_uint(c[4 * i + 2]), __float_as_uint(c[4 * i + 3]), 0x0040), 0x5410);
+  return make_uint2(w[0], w[1]);
+}
+
+// THREADS threads to a row, 256 / THREADS rows to a CTA; KEEP: vectors of 8 that a thread keeps.  VEC: rows of whole vectors.
+template <int THREADS, int KEEP, bool VEC, typename T>
+__global__ void __launch_bounds__(256)
+    quantize_rows_kernel(const T* __restrict__ x, size_t ldx, long long rows, int n, int8_t* __restrict__ q,
+                         size_t ldq, float* __restrict__ scale) {
+  __shared__ float s_top[8];
+  const int tid = threadIdx.x % THREADS;
+  const long long r = static_cast<long long>(blockIdx.x) * (256 / THREADS) + threadIdx.x / THREADS;
+  if (r >= rows) return;  // whole warps
+  griddep_wait();
+  griddep_launch_dependents();
+  const T* xr = x + r * ldx;
+  int8_t* qr = q + r * ldq;
+  const int whole = VEC ? n / 8 : 0;  // vectors; what is left is taken singly
+  float kept[KEEP][8], top = 0.f;
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int i = k * THREADS + tid;
+    if (i < whole) {
+      load8(xr + 8 * i, kept[k]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(kept[k][j]));
+    }
+  }
+  for (int i = KEEP * THREADS + tid; i < whole; i += THREADS) {
+    float f[8];
+    load8(xr + 8 * i, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(f[j]));
+  }
+  for (int i = 8 * whole + tid; i < n; i += THREADS) top = max_nan(top, fabsf(as_f32(xr[i])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (THREADS > 32) {
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) top = max_nan(top, s_top[w]);
+  }
+  const float s = top <= 3.402823466e38f ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fffffff);
+  if (tid == 0) scale[r] = s;
+  const bool some = s > 0.f;
+  const float per_s = __frcp_rn(some ? s : 1.f);
+  // a scale so small that its inverse is not a number's takes divisions
+  const bool tiny = !(per_s <= 3.0e38f);
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int i = k * THREADS + tid;
+    if (i < whole) *reinterpret_cast<uint2*>(qr + 8 * i) = some && !tiny ? codes8(kept[k], s, per_s) : make_uint2(0, 0);
+  }
+  for (int i = KEEP * THREADS + tid; i < whole; i += THREADS) {
+    float f[8];
+    load8(xr + 8 * i, f);
+    *reinterpret_cast<uint2*>(qr + 8 * i) = some && !tiny ? codes8(f, s, per_s) : make_uint2(0, 0);
+  }
+  for (int i = some && tiny ? tid : 8 * whole + tid; i < n; i += THREADS)
+    qr[i] = some ? static_cast<int8_t>(rintf(__fdiv_rn(as_f32(xr[i]), s))) : 0;
+}
+
+template <typename T>
+int quantize_run(const T* x, size_t ldx, size_t rows, int n, int8_t* q, size_t ldq, float* scale, cudaStream_t st) {
+  const bool vec = aligned16(x) && (rows == 1 || ldx * sizeof(T) % 16 == 0) &&
+                   (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && (rows == 1 || ldq % 8 == 0);
+  const auto go = [&](auto kernel, int per) {
+    return launch_pdl(kernel, dim3(ceil_div(rows, per)), dim3(256), 0, st, "quantize_rows_kernel", x, ldx,
+                      static_cast<long long>(rows), n, q, ldq, scale);
+  };
+  // a warp holds rows of up to 1024 values; longer ones, and rows too few to fill the GPU by warps, take a CTA
+  const bool cta = n > 1024 || (n > 256 && rows < static_cast<size_t>(8 * sm_count()));
+  if (!vec) return cta ? go(quantize_rows_kernel<256, 1, false, T>, 1) : go(quantize_rows_kernel<32, 1, false, T>, 8);
+  return cta ? go(quantize_rows_kernel<256, 2, true, T>, 1) : go(quantize_rows_kernel<32, 4, true, T>, 8);
 }
 
 // ----------------------------------------------------------------- products
@@ -389,12 +473,8 @@ int gsvk_quantize_rows_i8(const void* x, int is_f32, size_t rows, size_t n, size
   if (!ldq) ldq = n;
   if (rows > 1 && (ldx < n || ldq < n)) return fail(GSVK_ERR_INVALID, "quantize_rows_i8: leading dimension below %zu", n);
   if (n > 0x7fffffc0 || rows > 0x7fffffff) return fail(GSVK_ERR_UNSUPPORTED, "quantize_rows_i8: too big");
-  const unsigned blocks = ceil_div(rows, 8);
-  if (is_f32)
-    quantize_rows_kernel<<<blocks, 256, 0, as_cuda(stream)>>>(static_cast<const float*>(x), ldx, rows, (int)n, q, ldq, scale);
-  else
-    quantize_rows_kernel<<<blocks, 256, 0, as_cuda(stream)>>>(static_cast<const uint16_t*>(x), ldx, rows, (int)n, q, ldq, scale);
-  return check_launch("quantize_rows_kernel");
+  return is_f32 ? quantize_run(static_cast<const float*>(x), ldx, rows, (int)n, q, ldq, scale, as_cuda(stream))
+                : quantize_run(static_cast<const uint16_t*>(x), ldx, rows, (int)n, q, ldq, scale, as_cuda(stream));
 }
 
 int gsvk_gemm_i8(const gsvk_gemm_i8_args* g, gsvk_stream_t stream) {

@@ -62,16 +62,6 @@ __device__ __forceinline__ void load8(const uint16_t* p, float* f, float* lo, fl
   *lo = __low2float(m);
   *hi = -__high2float(m);
 }
-__device__ __forceinline__ float min_nan(float x, float y) {
-  float m;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
-  return m;
-}
-__device__ __forceinline__ float max_nan(float x, float y) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
-  return m;
-}
 template <int L>
 __device__ __forceinline__ void load8(const float* p, float* f, float* lo, float* hi) {
   const uint4 a = ld_stream_u4(p), b = ld_stream_u4(p + 4);
