@@ -188,6 +188,31 @@ __device__ __forceinline__ uint8_t* unit16(uint8_t* tile, int r, int j) {
   return tile + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
 }
 
+// GELU of 32 values, two to an operation: gelu_erf's Phi(-u) (common.cuh) as x Phi(x) = max(x, 0) - |x| Phi(-|x|).
+__device__ __forceinline__ void gelu32(float* v) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const uint64_t x = pair(v[j], v[j + 1]), u = pair(fminf(fabsf(v[j]), 5.5f), fminf(fabsf(v[j + 1]), 5.5f));
+    uint64_t h = pair(-1.725302567e-08f, -1.725302567e-08f);
+    h = fma2(h, u, pair(5.477549507e-07f, 5.477549507e-07f));
+    h = fma2(h, u, pair(-7.458289474e-06f, -7.458289474e-06f));
+    h = fma2(h, u, pair(5.484473149e-05f, 5.484473149e-05f));
+    h = fma2(h, u, pair(-2.005067072e-04f, -2.005067072e-04f));
+    h = fma2(h, u, pair(-1.761470485e-04f, -1.761470485e-04f));
+    h = fma2(h, u, pair(7.180649787e-03f, 7.180649787e-03f));
+    h = fma2(h, u, pair(-5.261564627e-02f, -5.261564627e-02f));
+    h = fma2(h, u, pair(2.621913850e-01f, 2.621913850e-01f));
+    h = fma2(h, u, pair(-1.151113272e+00f, -1.151113272e+00f));
+    h = fma2(h, u, pair(-9.999998212e-01f, -9.999998212e-01f));
+    const float2 e = unpair(fma2(mul2(x, x), pair(-0.721347520444f, -0.721347520444f), h));
+    float q0, q1;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(e.y));
+    v[j] = fmaf(-fabsf(v[j]), q0, max_nan(v[j], 0.f));
+    v[j + 1] = fmaf(-fabsf(v[j + 1]), q1, max_nan(v[j + 1], 0.f));
+  }
+}
+
 template <int BN>
 __global__ void __launch_bounds__(kI8Threads<BN>, 1)
     gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -239,47 +264,59 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      int s = 0, loaded = 0;
+      uint32_t ph = 1;
       bool ok = true;
       for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
         const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
-        for (int kb = 0; kb < kbn; ++kb, ++it) {
-          const int s = it % p.stages;
-          if (!mbar_wait(&empty[s], (static_cast<uint32_t>(it / p.stages) & 1u) ^ 1u, status)) {
+        for (int kb = 0; kb < kbn; ++kb) {
+          if (!mbar_wait(&empty[s], ph, status)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
           tma_load_2d(sA + s * kABytes, &tmA, &full[s], kb * kI8BK, mt * kI8BM);
           tma_load_2d(sB + s * kBBytes, &tmB, &full[s], kb * kI8BK, nt * BN);
+          loaded = min(loaded + 1, p.stages);
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
       }
-      if (!ok)  // a wait ran out: leave once the loads in flight have landed
-        for (int i = max(0, it - p.stages); i < it; ++i)
-          mbar_wait(&full[i % p.stages], static_cast<uint32_t>(i / p.stages) & 1u, status);
+      // A wait ran out: leave once the loads in flight have landed (the last use of each stage, newest last).
+      for (int i = 0; !ok && i < loaded; ++i) {
+        const int last = s - 1 - i;
+        mbar_wait(&full[last < 0 ? last + p.stages : last], last < 0 ? ph : ph ^ 1u, status);
+      }
     }
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8(kI8BM, BN);
-      int it = 0, tl = 0;
+      // descriptors of stage 0; others lie at offsets in 16 bytes
+      const uint64_t a0 = smem_desc(smem_u32(sA), 1024, 2), b0 = smem_desc(smem_u32(sB), 1024, 2);
+      int s = 0, tl = 0;
+      uint32_t ph = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++tl) {
         const int acc = tl & 1;
         if (!mbar_wait(&tempty[acc], (static_cast<uint32_t>(tl >> 1) & 1u) ^ 1u, status)) break;
         tc_fence_after();
-        for (int kb = 0; kb < kbn; ++kb, ++it) {
-          const int s = it % p.stages;
-          if (!mbar_wait(&full[s], static_cast<uint32_t>(it / p.stages) & 1u, status)) {
+        for (int kb = 0; kb < kbn; ++kb) {
+          if (!mbar_wait(&full[s], ph, status)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a = smem_u32(sA + s * kABytes), b = smem_u32(sB + s * kBBytes);
+          const uint64_t a = a0 + s * (kABytes / 16), b = b0 + s * (kBBytes / 16);
 #pragma unroll
           for (int j = 0; j < kI8BK / 32; ++j)
-            tc_mma_i8(tmem + acc * BN, smem_desc(a + 32u * j, 1024, 2), smem_desc(b + 32u * j, 1024, 2), idesc,
-                      (kb | j) ? 1u : 0u);
+            tc_mma_i8(tmem + acc * BN, a + 2 * j, b + 2 * j, idesc, (kb | j) ? 1u : 0u);
           tc_commit(&empty[s]);
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
         if (ok) tc_commit(&tfull[acc]);
       }
@@ -321,10 +358,16 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           const float4 c = *reinterpret_cast<const float4*>(&s_col[w][j]);
-          v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])), sa * c.x, c.y);
-          v[j + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + 1])), sa * c.z, c.w);
+          const uint64_t a2 = pair(static_cast<float>(static_cast<int>(r[j])), static_cast<float>(static_cast<int>(r[j + 1])));
+          const float2 y = unpair(fma2(a2, mul2(pair(sa, sa), pair(c.x, c.z)), pair(c.y, c.w)));
+          v[j] = y.x;
+          v[j + 1] = y.y;
         }
-        act_array<32>(v, e.act, e.slope);
+        if (e.act == GSVK_ACT_GELU_ERF) {
+          gelu32(v);
+        } else {
+          act_array<32>(v, e.act, e.slope);
+        }
         if (e.residual && row < p.M) {
           const float* res = e.residual + row * e.ld_res + n0;
 #pragma unroll
