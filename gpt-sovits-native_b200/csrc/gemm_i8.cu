@@ -155,13 +155,16 @@ constexpr int kI8BM = 128;
 constexpr int kI8BK = 128;  // bytes of K per stage
 constexpr int kI8MaxStages = 8;
 
+// Four epilogue warps (a tile's rows) to every 32 columns, at most 16: with 8 at 256 columns the epilogue took twice as
+// long as the products (encoder layer with GELU: 34 against 17 us).
 template <int BN>
-constexpr int kI8EpiWarps = BN >= 128 ? 8 : 4;  // two column halves from 128 columns on
+constexpr int kI8EpiWarps = BN >= 128 ? 16 : BN / 8;
 template <int BN>
 constexpr int kI8Threads = 64 + 32 * kI8EpiWarps<BN>;
 
 struct I8Problem {
   int M, N, K, m_tiles, n_tiles, stages;
+  int buffers;       // staged tiles of an epilogue warp and type: 1 or 2
   int tma32, tma16;  // outputs that leave by TMA
 };
 
@@ -188,10 +191,10 @@ __device__ __forceinline__ uint8_t* unit16(uint8_t* tile, int r, int j) {
   return tile + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
 }
 
-// GELU of 32 values, two to an operation: gelu_erf's Phi(-u) (common.cuh) as x Phi(x) = max(x, 0) - |x| Phi(-|x|).
-__device__ __forceinline__ void gelu32(float* v) {
+// GELU of 16 values, two to an operation: gelu_erf's Phi(-u) (common.cuh) as x Phi(x) = max(x, 0) - |x| Phi(-|x|).
+__device__ __forceinline__ void gelu16(float* v) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int j = 0; j < 16; j += 2) {
     const uint64_t x = pair(v[j], v[j + 1]), u = pair(fminf(fabsf(v[j]), 5.5f), fminf(fabsf(v[j + 1]), 5.5f));
     uint64_t h = pair(-1.725302567e-08f, -1.725302567e-08f);
     h = fma2(h, u, pair(5.477549507e-07f, 5.477549507e-07f));
@@ -227,8 +230,8 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
   uint8_t* smem = align_smem<1024>(i8_raw);
   uint8_t* sA = smem;
   uint8_t* sB = sA + p.stages * kABytes;
-  uint8_t* sOut = sB + p.stages * kBBytes;  // per epilogue warp: two fp32 and two fp16 tiles, as far as needed
-  const int out_bytes = 2 * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
+  uint8_t* sOut = sB + p.stages * kBBytes;  // per epilogue warp: fp32 and fp16 tiles, as far as needed
+  const int out_bytes = p.buffers * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
   __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], tfull[2], tempty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float2 s_col[kEpi][32];  // column scale and bias of a warp's chunk
@@ -323,10 +326,10 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
     }
   } else {
     const int w = warp - 2, quarter = warp & 3;  // TMEM lanes 32 quarter .. + 31
-    constexpr int kSpan = kEpi == 8 ? BN / 2 : BN;
-    const int cbeg = kEpi == 8 ? (w >> 2) * kSpan : 0;
+    constexpr int kSpan = BN / (kEpi / 4);
+    const int cbeg = (w >> 2) * kSpan;
     uint8_t* out32 = sOut + w * out_bytes;
-    uint8_t* out16 = out32 + (e.c32 ? 2 * kI8Tile32 : 0);
+    uint8_t* out16 = out32 + (e.c32 ? p.buffers * kI8Tile32 : 0);
     int turn = 0, tl = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++tl) {
       const int mt = tile / p.n_tiles, nt = tile - mt * p.n_tiles;
@@ -346,47 +349,55 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
         if (n0 >= p.N) break;
         s_col[w][lane] = col;
         if (c0 + 32 < cbeg + kSpan) col = column(c0 + 32);
-        uint32_t r[32];
+        uint8_t* t32 = out32 + (turn & (p.buffers - 1)) * kI8Tile32;
+        uint8_t* t16 = out16 + (turn & (p.buffers - 1)) * kI8Tile16;
         const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + c0;
-        tmem_ld16(from, r);
-        tmem_ld16(from + 16, r + 16);
         // the stores that read this turn's tiles are done with them
-        if (lane == 0 && (p.tma32 || p.tma16)) bulk_wait_read<1>();
-        tmem_ld_wait();
+        if (lane == 0 && (p.tma32 || p.tma16)) {
+          if (p.buffers == 2) {
+            bulk_wait_read<1>();
+          } else {
+            bulk_wait_read<0>();
+          }
+        }
         __syncwarp();
-        float v[32];
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {  // 16 columns at a time
+          uint32_t r[16];
+          tmem_ld16(from + 16 * q, r);
+          tmem_ld_wait();
+          float v[16];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float4 c = *reinterpret_cast<const float4*>(&s_col[w][j]);
-          const uint64_t a2 = pair(static_cast<float>(static_cast<int>(r[j])), static_cast<float>(static_cast<int>(r[j + 1])));
-          const float2 y = unpair(fma2(a2, mul2(pair(sa, sa), pair(c.x, c.z)), pair(c.y, c.w)));
-          v[j] = y.x;
-          v[j + 1] = y.y;
-        }
-        if (e.act == GSVK_ACT_GELU_ERF) {
-          gelu32(v);
-        } else {
-          act_array<32>(v, e.act, e.slope);
-        }
-        if (e.residual && row < p.M) {
-          const float* res = e.residual + row * e.ld_res + n0;
+          for (int j = 0; j < 16; j += 2) {
+            const float4 c = *reinterpret_cast<const float4*>(&s_col[w][16 * q + j]);
+            const uint64_t a2 = pair(static_cast<float>(static_cast<int>(r[j])), static_cast<float>(static_cast<int>(r[j + 1])));
+            const float2 y = unpair(fma2(a2, mul2(pair(sa, sa), pair(c.x, c.z)), pair(c.y, c.w)));
+            v[j] = y.x;
+            v[j + 1] = y.y;
+          }
+          if (e.act == GSVK_ACT_GELU_ERF) {
+            gelu16(v);
+          } else {
+            act_array<16>(v, e.act, e.slope);
+          }
+          if (e.residual && row < p.M) {
+            const float* res = e.residual + row * e.ld_res + n0 + 16 * q;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (n0 + j < p.N) v[j] += res[j];
-        }
-        uint8_t* t32 = out32 + (turn & 1) * kI8Tile32;
-        uint8_t* t16 = out16 + (turn & 1) * kI8Tile16;
-        if (e.c32) {
+            for (int j = 0; j < 16; ++j)
+              if (n0 + 16 * q + j < p.N) v[j] += res[j];
+          }
+          if (e.c32) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(unit32(t32, lane, j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
-        if (e.c16) {
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(unit32(t32, lane, 4 * q + j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+          if (e.c16) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(unit16(t16, lane, j)) =
-                make_uint4(f2h2(v[8 * j], v[8 * j + 1]), f2h2(v[8 * j + 2], v[8 * j + 3]),
-                           f2h2(v[8 * j + 4], v[8 * j + 5]), f2h2(v[8 * j + 6], v[8 * j + 7]));
+            for (int j = 0; j < 2; ++j)
+              *reinterpret_cast<uint4*>(unit16(t16, lane, 2 * q + j)) =
+                  make_uint4(f2h2(v[8 * j], v[8 * j + 1]), f2h2(v[8 * j + 2], v[8 * j + 3]),
+                             f2h2(v[8 * j + 4], v[8 * j + 5]), f2h2(v[8 * j + 6], v[8 * j + 7]));
+          }
         }
         if (p.tma32 || p.tma16) fence_proxy_async_shared();
         __syncwarp();
@@ -460,8 +471,10 @@ int launch_i8(const gsvk_gemm_i8_args* g, size_t lda, size_t ldb, const I8Epilog
     p.tma16 = 1;
   }
   if (rc) return rc;
-  constexpr size_t kLimit = 227 * 1024 - 4096;  // barriers and column tables are static
-  const size_t staging = static_cast<size_t>(kI8EpiWarps<BN>) * 2 * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
+  constexpr size_t kLimit = 227 * 1024 - 6144;  // barriers and column tables are static
+  // one staged tile where fp32 ones would leave too little for the operands
+  p.buffers = e.c32 ? 1 : 2;
+  const size_t staging = static_cast<size_t>(kI8EpiWarps<BN>) * p.buffers * ((e.c32 ? kI8Tile32 : 0) + (e.c16 ? kI8Tile16 : 0));
   const size_t stage = (kI8BM + BN) * kI8BK;
   const int kbn = (p.K + kI8BK - 1) / kI8BK;
   p.stages = static_cast<int>(std::min<size_t>(kI8MaxStages, (kLimit - 1024 - staging) / stage));
