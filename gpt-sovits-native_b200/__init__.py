@@ -1120,3 +1120,4 @@ class T2SBatch:
 # --------------------------------- quantised serving: 4-bit KV cache, int8 layers
 from .quant import (  # noqa: E402,F401
     KV4Cache, KV4Workspace, KVPlan, gemm_i8, kv4_page_bytes, quantize_rows_i8)
+from .paged import Linear8, T2SPaged  # noqa: E402,F401
