@@ -6,34 +6,36 @@
 // persistent CTA per SM takes an equal run of the line of units (kv4_attn.cuh),
 // so no SM waits for the longest item, and the loads and the unpacking of an
 // item overlap the end of the last.  A run's first and last item may be shared with
-// other CTAs: the warp that finishes its 32 rows last joins the pieces.  (With a
-// CTA to an item, starting and ending them cost 126 of 390 us on 50 blocks of 16 heads.)  Roles:
-//   warps 0-3, 4-7  softmax of the first and the second block: a thread to a row (its TMEM lane)
-//   warps 8-11      unpack a tile's codes into fp16 operands
-//   warp 12         copies the tile's pages into shared memory (cp.async.bulk)
-//   warp 13         issues the MMAs:  S = Q K^T  and  O += W V, W from TMEM over the scores it came from
-// While the tensor cores work on one block's products, the other block's
-// softmax runs; what is unpacked serves both.
+// other CTAs: the warp that finishes its 32 rows last joins the pieces.  Roles:
+//   warps 0-3, 4-7    softmax of the first and the second block: a thread to a row (its TMEM lane)
+//   warps 8-11, 12-15 unpack a tile's keys and values into fp16 operands
+//   warp 16           copies the tile's pages into shared memory (cp.async.bulk)
+//   warp 17           issues the MMAs:  S = Q K^T  and  O += W V, W from TMEM over the scores it came from
+// The blocks' tiles take a ring of score tiles in TMEM in turn: three of 128
+// columns (head_dim 128: four of 64) beside the sums, so that a softmax finds its
+// next scores done while the other block's products run.  What is unpacked serves both.
 //
 // Mathematics.  k_j = a c + b (step, codes, low), so q.k_j = q.(a c) + sum(q) b.
 // a c takes 15 bits: it goes in as the sum of two fp16 numbers, one product
 // and one fused product for two codes, and b as one more column of K against
 // sum(q), which is two columns of Q.  So no score is rounded below fp32
 // (K as one fp16 number would move each by 2^-12 |q||k|).
-// v_j goes in as two fp16 parts at head_dim 32 and 64, side by side as
-// 2 head_dim columns of the value operand (an MMA of 128 x 128 takes the 67
-// clocks that one of 128 x 64 takes: measured).  At head_dim 128 that would double the MMAs:
+// v_j goes in as two fp16 parts at head_dim 32 and 64.  At head_dim 128 that would double the MMAs:
 //   sum_j p_j v_j = sum_j (p_j s_j) (e_j - 8) + sum_j p_j (f_j + 8 s_j)
 // there, with the codes e - 8 as the operand and the last sum in the softmax.
 // Either way the one rounding to fp16 beside the result's is that of the
 // weights: 2^-11 of the values (centred within 8 steps at head_dim 128).
-// p_j = 2^(z_j - reference); the reference is the row's maximum as of the last
-// time that it grew by 2^8: until then the weights stay in fp16's range and the
-// sums in TMEM are left alone.  K and V (s) are divided by a power of two, that
-// of K by tile, that of V the same for all rows.
+// p_j = 2^(z_j - reference).  The reference is the maximum of the item's first tile, and moves only when a sum of
+// weights shows that they outgrow fp16's range: so the maximum is taken once an item and the sums in TMEM are
+// mostly left alone.  K and V (s) are divided by a power of two, that of K by tile, that of V the same for all rows.
 //
-// What bounds it, per 256 x 128 scores at head_dim 64: 2 x (9 + 8) MMAs of 67 clocks = 2,278, 32,768
-// exponentials at 16 a clock = 2,048, 5,400 warp instructions at 4 a clock.
+// What bounds it, per 256 x 128 scores at head_dim 64: 2 x (9 + 16) MMAs of 67 clocks = 3,350, and 32,768
+// exponentials at 16 a clock = 2,048; a softmax warp takes 3,100 clocks for its 32 x 128 and some 7,000 between
+// items.  Measured at 320 us on four prompts of 2,000 to 4,096 tokens, 16 heads of 64 (16,200 such tiles, 5,000
+// clocks each); 400 us with one score tile a block, whose softmax waited for its products, and unpacking on four warps;
+// 372 us with the codes as the value operand as at head_dim 128 (fewer MMAs, more work in the softmax); 385 us
+// with the maximum taken of every tile.  The MMAs are issued by an elected lane of a converged warp: from
+// inside a lane's own branch, where descriptors cannot stay in uniform registers, each took 122 clocks instead of 78.
 #include <algorithm>
 
 #include "gsvk_internal.hpp"
@@ -44,19 +46,24 @@ namespace gsvk {
 namespace {
 
 constexpr int kPBlock = 128, kPRows = 2 * kPBlock;  // rows of a softmax group and of a CTA
-constexpr int kPThreads = 512;
-constexpr int kPRegs = 128, kPRegsSoftmax = 152, kPRegsUnpack = 96, kPRegsRest = 112;
-static_assert(2 * kPRegsSoftmax + kPRegsUnpack + kPRegsRest <= 4 * kPRegs, "register shares exceed the launch's");
+constexpr int kPThreads = 576;  // 112 registers each
 constexpr uint32_t kPTmemCols = 512;
 
 template <int HD>
-constexpr bool kPSplit = HD <= 64;  // values as two fp16 numbers
+constexpr bool kPSplit = HD <= 64;  // values as two fp16 numbers (the time of either form is above)
 template <int HD>
 constexpr int kPTile = HD <= 64 ? 128 : 64;  // keys
 template <int HD>
 constexpr int kPTileShift = HD <= 64 ? 7 : 6;
 template <int HD>
-constexpr int kPCols = kPSplit<HD> ? 2 * HD : HD;  // columns of the value operand and of the sums
+constexpr bool kPSide = HD == 32;  // their parts side by side, in sums of their own; else both into the same sums
+template <int HD>
+constexpr int kPCols = kPSplit<HD> ? 2 * HD : HD;  // columns of the value operand
+template <int HD>
+constexpr int kPSums = kPSide<HD> ? 2 * HD : HD;  // and of the sums
+template <int HD>
+constexpr int kPRing = kPTile<HD> == 128 ? 3 : 4;  // tiles of scores in TMEM
+constexpr int kPPar = 3;  // tiles of parameters: no more than of scores, so that no group lags by a round
 
 // What the softmax needs of a tile's keys.
 template <int HD>
@@ -80,7 +87,7 @@ template <int HD>
 constexpr int kPRawBytes = kPTile<HD> * (HD + 8);
 template <int HD>
 constexpr int kPSmem = 1024 + kPQBytes<HD> + kPRows * 32 + 2 * kPKeyBytes<HD> + 2 * kPValBytes<HD> + kPRaw * kPRawBytes<HD> +
-                       2 * static_cast<int>(sizeof(TileParams<HD>));
+                       kPPar * static_cast<int>(sizeof(TileParams<HD>));
 
 // 16-byte unit u of row r of an operand tile with COLS columns: rows of 64 values in the 128-byte swizzle, 128
 // columns as two slabs of `rows` rows, 32 as 64-byte rows in the 64-byte swizzle.
@@ -103,13 +110,24 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b
       "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+// One lane of the warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Waits for two phases, asked for at once: what each takes when it is there is a latency, some 100 clocks beside the
+// other warps.
+__device__ __forceinline__ bool wait_for(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py, uint32_t* status) {
+  const bool there = mbar_try_wait(x, px) & mbar_try_wait(y, py);
+  return there || (mbar_wait(x, px, status) && mbar_wait(y, py, status));
+}
+// A value that is the same in every lane, known to be so.
+__device__ __forceinline__ int same(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
@@ -117,23 +135,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// N consecutive words of shared memory, in as few loads as they allow (aligned to their size, at most 16 bytes).
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
-      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-    }
-  }
-}
 
 // Eight codes w of a row, times s, as the sum of two fp16 numbers, in the order of the word's nibbles:
 // 0 4, 1 5, 2 6, 3 7.
@@ -246,7 +247,9 @@ __device__ __forceinline__ void put8(uint16_t* out, const float* v) {
 template <int HD>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs a) {
   constexpr int kT = kPTile<HD>, kTs = kPTileShift<HD>;
-  constexpr uint32_t kO = 256;  // TMEM column of the sums: block 0 there, block 1 at + 128; scores of block b at 128 b
+  constexpr int kR = kPRing<HD>;
+  constexpr uint32_t kO = kR * kT;  // TMEM column of the sums, block after block; below, the ring of scores
+  static_assert(kO + 2 * kPSums<HD> <= kPTmemCols);
   using L = PromptLine<HD>;
   extern __shared__ uint8_t prompt_raw[];
   uint8_t* smem = align_smem<1024>(prompt_raw);
@@ -258,14 +261,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
   TileParams<HD>* par = reinterpret_cast<TileParams<HD>*>(sRaw + kPRaw * kPRawBytes<HD>);
   // Buffers of a tile, which the tiles of a run take in turn whatever their item,
   __shared__ uint64_t raw_full[kPRaw], raw_free[kPRaw], k_full[2], k_free[2], v_full[2], v_free[2];
-  __shared__ uint64_t par_full[2], par_free[2], most_full[2];
-  // and what belongs to a block of rows: a phase for each of its tiles, or of its items.
-  __shared__ uint64_t s_full[2], p_half[2], p_full[2], q_full[2], o_full[2], o_free[2];
+  __shared__ uint64_t par_full[kPPar], par_free[kPPar], most_full[2][2];
+  // the scores and weights of a block's tile, which take the ring in turn,
+  __shared__ uint64_t s_full[kR], p_full[kR];
+  // and what belongs to a block of rows: a phase for each of its items, o_tile for each of its tiles.
+  __shared__ uint64_t q_full[2], o_full[2], o_free[2], o_tile[2];
   __shared__ uint32_t raw_ok[kPRaw];
-  __shared__ __align__(16) float2 s_most[2][4];
+  __shared__ __align__(16) float s_most[2][2][4];
   __shared__ uint32_t tmem_slot;
   __shared__ typename L::template Runs<kPThreads> runs;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = same(tid >> 5), lane = tid & 31;
 
   L::template measure<kPThreads>(a, runs, static_cast<int>(gridDim.x), kPMaxPieces);
   const int me = static_cast<int>(blockIdx.x);
@@ -277,26 +282,31 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
   if (tid == 0) {
     for (int i = 0; i < kPRaw; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 4);
+      mbar_init(&raw_free[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&k_free[i], 1);
       mbar_init(&v_full[i], 4);
       mbar_init(&v_free[i], 1);
-      mbar_init(&par_full[i], 4);
-      mbar_init(&par_free[i], 8);
-      mbar_init(&most_full[i], 4);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&p_half[i], 4);
+      mbar_init(&most_full[0][i], 4);
+      mbar_init(&most_full[1][i], 4);
       mbar_init(&q_full[i], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 4);
+      mbar_init(&o_tile[i], 1);
+    }
+    for (int i = 0; i < kPPar; ++i) {
+      mbar_init(&par_full[i], 8);
+      mbar_init(&par_free[i], 8);
+    }
+    for (int i = 0; i < kR; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
     }
     fence_barrier_init();
   }
-  if (warp == 13) {
+  if (warp == 17) {
     tmem_alloc(&tmem_slot, kPTmemCols);
     tmem_relinquish();
   }
@@ -314,11 +324,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsSoftmax));
     const int block = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t scores = tmem + lanes + block * 128, sums = tmem + lanes + kO + block * 128;
+    const uint32_t sums = tmem + lanes + kO + block * kPSums<HD>;
     int mine = 0, items = 0;  // this block's tiles and items so far
+    int slot = 0;  // the ring's turn of the item's first tile, its place and the parity of its round
+    uint32_t round = 0;
+    const auto advance = [&](int n) {
+      slot += n;
+      if (slot >= kR) slot -= kR, round ^= 1u;
+    };
     int item_start = -at.tile;
     bool ok = true;
     const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // scores are taken with a positive scale
@@ -330,43 +345,47 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       if (lane == 0) mbar_arrive(&q_full[block]);
     }
     while (g < run && ok) {
-
       const int all = at.req.n * a.group, row = at.block * kPRows + tid;
-      const bool live_row = row < all, active = block < blocks_of(at);
+      const int blocks = blocks_of(at);
+      const bool live_row = row < all, active = block < blocks;
       const int limit = limit_of(a, at.req, min(row, all - 1));
       const int least = __reduce_min_sync(0xffffffffu, limit);
       const int t0 = at.tile, t1 = min(at.tiles, t0 + run - g);
-      float ref = -INFINITY, unit = 0.f;
+      float ref = -INFINITY, unit = 0.f, tile_sum = 0.f;
       uint64_t l2 = 0, pb2 = 0;
       for (int i = t0; i < t1; ++i, ++g) {
-        const TileParams<HD>& t = par[g & 1];
-        ok = mbar_wait(&par_full[g & 1], static_cast<uint32_t>(g >> 1) & 1u, a.status) &&
-             (!active || mbar_wait(&s_full[block], static_cast<uint32_t>(mine) & 1u, a.status));
+        const TileParams<HD>& t = par[g % kPPar];
+        // Its own scores' place; a group without rows waits for the first block's: nobody may fall a round of the ring
+        // behind or get one ahead, where a phase has the parity of another.
+        if (active && block) advance(1);
+        const int here = slot;
+        ok = wait_for(&par_full[g % kPPar], static_cast<uint32_t>(g / kPPar) & 1u, &s_full[here], round, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (!active) {
-          if (lane == 0) mbar_arrive(&par_free[g & 1]);
+          advance(1);
+          if (lane == 0) mbar_arrive(&par_free[g % kPPar]);
           continue;
         }
-        ++mine;
+        advance(blocks - block);
+        const uint32_t scores = tmem + lanes + here * kT;
         tc_fence_after();
-        const float score = t.score, rescale = t.rescale;
+        const float score = t.score;
         const uint32_t page_ok = t.page_ok;
         unit = t.unit;
-        // Two passes over the scores in loops of a few dozen instructions: three roles share the instruction caches.
+        // Loops of some dozen instructions: the roles share the instruction caches.
         const bool mask = i * kT + kT > least || page_ok != (1u << subs) - 1u;
         const int see = limit - i * kT;
-        // The 16 scores of a lane that keys c .. c + 15 have (one page's), hidden ones as minus infinity.
+        // 16 scores r of keys c .. c + 15 (one page's): hidden ones as minus infinity.
         const auto hide = [&](int c, uint32_t* r) {
           const int n = (page_ok >> (c >> sub_shift) & 1u) ? see - c : 0;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (j >= n) r[j] = 0xff800000u;
         };
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c = 0; c < kT; c += 32) {
-          uint32_t r[32];
+        // Scores c .. c + kChunk - 1 into r.
+        constexpr int kChunk = 32;
+        const auto fetch = [&](int c, uint32_t* r) {
           tmem_ld16(scores + c, r);
           tmem_ld16(scores + c + 16, r + 16);
           tmem_ld_wait();
@@ -374,75 +393,129 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
             hide(c, r);
             hide(c + 16, r + 16);
           }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2)
-            tops[(j >> 1) & 3] = fmaxf(fmaxf(tops[(j >> 1) & 3], __uint_as_float(r[j])), __uint_as_float(r[j + 1]));
-        }
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * score;
-        if (i == t0) {
-          ref = top;
-        } else if (__any_sync(0xffffffffu, top > ref + 8.f || rescale != 1.f)) {
-          // a new reference or unit: bring the sums to it (these scores were issued after the last sums)
-          const float to = fmaxf(ref, top);
-          const float keep = to == -INFINITY ? 1.f : ex2(ref - to);
-          ref = to;
-          l2 = mul2(l2, pair(keep, keep));
-          pb2 = mul2(pb2, pair(keep, keep));
-          const float by = keep * rescale;
+        };
+        // The reference is the first tile's maximum.  It follows a tile late when a tile's sum has passed 2^8, or at once
+        // when that of a chunk passes 2^15: every weight stays in fp16's range with no maximum to take of each tile.
+        float rescale = t.rescale;
+        bool follow = i == t0 || __any_sync(0xffffffffu, tile_sum > 256.f || rescale != 1.f);
+        float to = ref;
+        if (tile_sum > 256.f) to += static_cast<float>(static_cast<int>(__float_as_uint(tile_sum) >> 23) - 127);
+        tile_sum = 0.f;
+        int c = 0;
+        bool at_once = i == t0;
+        for (;;) {
+          if (follow) {
+            if (at_once) {  // the maximum of what is left of the tile
 #pragma unroll 1
-          for (int c = 0; c < kPCols<HD>; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(sums + c, o);
-            tmem_ld_wait();
+              for (int k = c; k < kT; k += kChunk) {
+                uint32_t r[kChunk];
+                fetch(k, r);
+                float x[4] = {to, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-            tmem_st16(sums + c, o);
-          }
-          tmem_st_wait();
-        }
-        const float base = ref == -INFINITY ? 0.f : ref;
-        const uint64_t nb = pair(-base, -base), sc = pair(score, score);
-        uint64_t more = 0;  // a second sum: the distance between dependent additions
+                for (int j = 0; j < kChunk; j += 2)
+                  x[(j >> 1) & 3] = fmaxf(fmaxf(x[(j >> 1) & 3], __uint_as_float(r[j]) * score),
+                                          __uint_as_float(r[j + 1]) * score);
+                to = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+              }
+            }
+            if (i == t0) {
+              ref = to;
+            } else {
+              // Bring the sums to the new reference or unit, once the last tile's products are in them (those of the one
+              // before are: these scores were issued after them), and this tile's weights so far: by a power of two.
+              ok = mbar_wait(&o_tile[block], static_cast<uint32_t>(mine - 1) & 1u, a.status);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
+              to = to > ref ? (ref == -INFINITY ? to : ref + ceilf(to - ref)) : ref;
+              const float keep = to == -INFINITY ? 1.f : ex2(ref - to);
+              ref = to;
+              tile_sum *= keep;
+              l2 = mul2(l2, pair(keep, keep));
+              pb2 = mul2(pb2, pair(keep, keep));
+              const float by = keep * rescale;
 #pragma unroll 1
-        for (int c = 0; c < kT; c += 16) {
-          uint32_t r[16], w[8];
-          tmem_ld16(scores + c, r);
-          tmem_ld_wait();
-          if (mask) hide(c, r);
+              for (int k = 0; k < kPSums<HD>; k += 8) {
+                uint32_t o[8];
+                tmem_ld8(sums + k, o);
+                tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 d = unpair(fma2(pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sc, nb));
-            const float2 e = make_float2(ex2(d.x), ex2(d.y));
-            const uint64_t p = pair(e.x, e.y);
-            if (j & 1) {
-              more = add2(more, p);
-            } else {
-              l2 = add2(l2, p);
-            }
-            if constexpr (kPSplit<HD>) {
-              w[j] = f2h2(e.x, e.y);
-            } else {
-              pb2 = fma2(p, *reinterpret_cast<const uint64_t*>(t.f + c + 2 * j), pb2);
-              const float2 x = unpair(mul2(p, *reinterpret_cast<const uint64_t*>(t.s + c + 2 * j)));
-              w[j] = f2h2(x.x, x.y);
+                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+                tmem_st8(sums + k, o);
+              }
+#pragma unroll 1
+              for (int k = 0; k < c / 2; k += 8) {
+                uint32_t w[8];
+                tmem_ld8(scores + k, w);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  w[j] = f2h2(h2f(static_cast<uint16_t>(w[j])) * keep, h2f(static_cast<uint16_t>(w[j] >> 16)) * keep);
+                tmem_st8(scores + k, w);
+              }
+              tmem_st_wait();
             }
           }
-          tmem_st8(scores + c / 2, w);  // over scores that have been read
-          if (kT == 128 && c == 48) {   // half of the weights: their products may begin
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_half[block]);
+          // a row that has seen nothing yet: weights without end for all that it sees, which sets its reference
+          const bool none = ref == -INFINITY;
+          const float nbase = none ? 1.0e38f : -ref, high = none ? 0.f : 32768.f;
+          const uint64_t nb = pair(nbase, nbase), sc = pair(score, score);
+          follow = false;
+#pragma unroll 1
+          for (; c < kT; c += kChunk) {
+            uint32_t r[kChunk], w[kChunk / 2];
+            fetch(c, r);
+            uint64_t even = 0, odd = 0;  // two sums: the distance between dependent additions
+#pragma unroll
+            for (int j = 0; j < kChunk / 2; ++j) {
+              const float2 d = unpair(fma2(pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), sc, nb));
+              const float2 e = make_float2(ex2(d.x), ex2(d.y));
+              const uint64_t p = pair(e.x, e.y);
+              if (j & 1) {
+                odd = add2(odd, p);
+              } else {
+                even = add2(even, p);
+              }
+              if constexpr (kPSplit<HD>) {
+                w[j] = f2h2(e.x, e.y);
+              } else {
+                const float2 x = unpair(mul2(p, *reinterpret_cast<const uint64_t*>(t.s + c + 2 * j)));
+                w[j] = f2h2(x.x, x.y);
+                r[2 * j] = __float_as_uint(e.x), r[2 * j + 1] = __float_as_uint(e.y);
+              }
+            }
+            even = add2(even, odd);
+            const float2 s2 = unpair(even);
+            const float sum = s2.x + s2.y;
+            if (__any_sync(0xffffffffu, sum > high)) {
+              follow = true;
+              break;
+            }
+            tile_sum += sum;
+            if constexpr (!kPSplit<HD>) {
+#pragma unroll
+              for (int j = 0; j < kChunk / 2; ++j)
+                pb2 = fma2(pair(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])),
+                           *reinterpret_cast<const uint64_t*>(t.f + c + 2 * j), pb2);
+            }
+            tmem_st8(scores + c / 2, w);
+            tmem_st8(scores + c / 2 + 8, w + 8);
           }
+          if (!follow) break;
+          rescale = 1.f;
+          to = ref;
+          at_once = true;
         }
-        l2 = add2(l2, more);
+        l2 = add2(l2, pair(tile_sum, 0.f));
+        if (!ok) break;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&p_full[block]);
-          mbar_arrive(&par_free[g & 1]);
+          mbar_arrive(&p_full[here]);
+          mbar_arrive(&par_free[g % kPPar]);
         }
+        ++mine;
       }
       if (!ok) break;
       // the next item's queries, over those that the last scores have used, while the last sums are made
@@ -477,7 +550,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
         tmem_ld16(sums + c, o);
-        if constexpr (kPSplit<HD>) {
+        if constexpr (kPSide<HD>) {
           uint32_t second[16];
           tmem_ld16(sums + HD + c, second);
           tmem_ld_wait();
@@ -552,15 +625,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       }
     }
     tc_fence_before();
-  } else if (warp < 12) {
-    // ----------------------------------------------------------------- unpack
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsUnpack));
-    constexpr int kPer = 128 / kT;           // threads to a key
-    constexpr int kWords = HD / 8 / kPer;    // words of codes of a thread
-    constexpr int kStep = 1;
-    const int me_key = tid - 256, key = me_key / kPer, part = me_key % kPer;
+  } else if (warp < 16) {
+    // ----------------------------------------------------------------- unpack: warps 8-11 the keys, 12-15 the values
+    constexpr int kPer = 128 / kT;         // threads to a key
+    constexpr int kWords = HD / 8 / kPer;  // words of codes of a thread
+    const int v = warp >= 12;              // 1: the values
+    const int me_key = (tid - 256) & 127, key = me_key / kPer, part = me_key % kPer;
     const int sub_bytes = kv4_head_bytes(sub_shift, HD), sub_mask = (1 << sub_shift) - 1;
     const int at_sub = (key >> sub_shift) * sub_bytes, at_key = key & sub_mask;
+    const int at_codes = at_sub + (v ? kv4_v_codes(sub_shift, HD) : 0) + at_key * (HD / 2) + part * (kWords * 4);
     bool ok = true;
     while (g < run && ok) {
       float unit = 0.f, per_unit = 0.f;
@@ -568,129 +641,118 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       for (int i = at.tile; i < t1; ++i, ++g) {
         const int rs = g % kPRaw, buf = g & 1;
         const uint32_t ph = static_cast<uint32_t>(g >> 1) & 1u;
-        ok = mbar_wait(&raw_full[rs], static_cast<uint32_t>(g / kPRaw) & 1u, a.status) &&
-             mbar_wait(&k_free[buf], ph ^ 1u, a.status) && mbar_wait(&par_free[buf], ph ^ 1u, a.status);
+        ok = wait_for(&raw_full[rs], static_cast<uint32_t>(g / kPRaw) & 1u, &par_free[g % kPPar],
+                      (static_cast<uint32_t>(g / kPPar) & 1u) ^ 1u, a.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t page_ok = raw_ok[rs];
         const uint8_t* sub = sRaw + rs * kPRawBytes<HD> + at_sub;
         const uint32_t kp = *reinterpret_cast<const uint32_t*>(sub + kv4_k_par(sub_shift, HD) + at_key * 4);
         const uint32_t vp = *reinterpret_cast<const uint32_t*>(sub + kv4_v_par(sub_shift, HD) + at_key * 4);
-        const uint8_t* key_codes = sub + at_key * (HD / 2) + part * (kWords * 4);
-        const uint8_t* value_codes = key_codes + kv4_v_codes(sub_shift, HD);
-        float ks = h2f(static_cast<uint16_t>(kp)), kl = h2f(static_cast<uint16_t>(kp >> 16));
-        float vs = h2f(static_cast<uint16_t>(vp)), vf = h2f(static_cast<uint16_t>(vp >> 16));
+        const uint8_t* codes = sRaw + rs * kPRawBytes<HD> + at_codes;
         // What lies past every row's limit or in a page that is not there counts as zero.  Keys or values that are
         // not numbers reach the rows that see them by their scores, which a row that does not see the key replaces.
         const bool seen = i * kT + key < keys && (page_ok >> (key >> sub_shift) & 1u);
-        const bool number = fabsf(ks) + fabsf(kl) + fabsf(vs) + fabsf(vf) <= 3.0e38f;
-        if (!seen || !number) ks = kl = vs = vf = 0.f;
-        // the units: the greatest key and value (or 16 steps; for head_dim 128 the greatest step) of the tile
+        const bool number = (kp & 0x7c00u) != 0x7c00u && (kp & 0x7c000000u) != 0x7c000000u && (vp & 0x7c00u) != 0x7c00u &&
+                            (vp & 0x7c000000u) != 0x7c000000u;
+        const uint32_t mine = !seen || !number ? 0u : v ? vp : kp;
+        const float step = h2f(static_cast<uint16_t>(mine)), low = h2f(static_cast<uint16_t>(mine >> 16));
+        // the unit: the greatest key or value (or 16 steps; of values at head_dim 128 the greatest step) of the tile
         {
-          const float mk = warp_max(fmaxf(fabsf(kl), 16.f * ks));
-          const float mv = warp_max(kPSplit<HD> ? fmaxf(fabsf(vf), 16.f * vs) : vs);
+          const float m = warp_max(v && !kPSplit<HD> ? step : fmaxf(fabsf(low), 16.f * step));
           if (lane == 0) {
-            s_most[buf][warp - 8] = make_float2(mk, mv);
-            mbar_arrive(&most_full[buf]);
+            s_most[v][buf][warp & 3] = m;
+            mbar_arrive(&most_full[v][buf]);
           }
-          ok = mbar_wait(&most_full[buf], ph, a.status);
+          ok = mbar_wait(&most_full[v][buf], ph, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        const float4 m0 = *reinterpret_cast<const float4*>(&s_most[buf][0]), m1 = *reinterpret_cast<const float4*>(&s_most[buf][2]);
-        const float most_k = fmaxf(fmaxf(m0.x, m0.z), fmaxf(m1.x, m1.z)), most_v = fmaxf(fmaxf(m0.y, m0.w), fmaxf(m1.y, m1.w));
-        float per_key;
-        const float key_unit = unit_above(most_k, &per_key);
-        float rescale = 1.f;  // the values' unit holds until something passes four times it
-        if (most_v > 4.f * unit) {
-          const float before = unit;
-          unit = unit_above(most_v, &per_unit);
-          rescale = before * per_unit;
-        }
-        uint8_t* keys_at = sK + buf * kPKeyBytes<HD>;
-        {
-          const __half2 s2 = __float2half2_rn(ks * per_key);
-#pragma unroll 1
-          for (int u = 0; u < kWords; u += kStep) {
-            uint32_t w[kStep];
-            load_words<kStep>(key_codes + 4 * u, w);
-#pragma unroll
-            for (int k = 0; k < kStep; ++k) {
-              uint4 first, second;
-              two_parts(w[k], s2, &first, &second);
-              const uint32_t to = unit_at<HD>(key, part * kWords + u + k, kT);
-              *reinterpret_cast<uint4*>(keys_at + to) = first;
-              *reinterpret_cast<uint4*>(keys_at + kPHalfBytes<HD> + to) = second;
-            }
+        const float4 m4 = *reinterpret_cast<const float4*>(&s_most[v][buf][0]);
+        const float most = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+        TileParams<HD>& t = par[g % kPPar];
+        if (!v) {
+          const float key_unit = unit_above(most, &per_unit);
+          if (me_key == 0) {
+            t.score = fmaxf(fabsf(a.scale_log2) * key_unit, 1e-30f);  // not 0, which a hidden score could not be scaled by
+            t.page_ok = page_ok;
           }
-        }
-        {
-          TileParams<HD>& t = par[buf];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&par_full[g % kPPar]);
+          ok = mbar_wait(&k_free[buf], ph ^ 1u, a.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint8_t* dst = sK + buf * kPKeyBytes<HD>;
+          const __half2 s2 = __float2half2_rn(step * per_unit);
+#pragma unroll 1
+          for (int u = 0; u < kWords; ++u) {
+            uint4 first, second;
+            two_parts(*reinterpret_cast<const uint32_t*>(codes + 4 * u), s2, &first, &second);
+            const uint32_t to = unit_at<HD>(key, part * kWords + u, kT);
+            *reinterpret_cast<uint4*>(dst + to) = first;
+            *reinterpret_cast<uint4*>(dst + kPHalfBytes<HD> + to) = second;
+          }
           if (part == 0) {
-            const float low = seen && !number ? __int_as_float(0x7fffffff) : kl * per_key;
-            put_two(keys_at + 2 * kPHalfBytes<HD>, key, low * 128.f, low * 0.0625f);
-            if constexpr (!kPSplit<HD>) {
-              t.s[key] = vs * per_unit;
-              t.f[key] = fmaf(8.f, vs, vf);
+            const float b = seen && !number ? __int_as_float(0x7fffffff) : low * per_unit;
+            put_two(dst + 2 * kPHalfBytes<HD>, key, b * 128.f, b * 0.0625f);
+          }
+        } else {
+          float rescale = 1.f;  // the values' unit holds until something passes four times it
+          if (most > 4.f * unit) {
+            const float before = unit;
+            unit = unit_above(most, &per_unit);
+            rescale = before * per_unit;
+          }
+          if constexpr (!kPSplit<HD>) {
+            if (part == 0) {
+              t.s[key] = step * per_unit;
+              t.f[key] = fmaf(8.f, step, low);
             }
           }
           if (me_key == 0) {
-            t.score = fmaxf(fabsf(a.scale_log2) * key_unit, 1e-30f);  // not 0, which a hidden score could not be scaled by
             t.unit = unit;
             t.rescale = rescale;
-            t.page_ok = page_ok;
           }
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&k_full[buf]);
-          mbar_arrive(&par_full[buf]);
-        }
-        ok = mbar_wait(&v_free[buf], ph ^ 1u, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&par_full[g % kPPar]);
+          ok = mbar_wait(&v_free[buf], ph ^ 1u, a.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           uint8_t* dst = sV + buf * kPValBytes<HD>;
-          const __half2 s2 = __float2half2_rn(vs * per_unit), low2 = __float2half2_rn(vf * per_unit);
+          const __half2 s2 = __float2half2_rn(step * per_unit), low2 = __float2half2_rn(low * per_unit);
 #pragma unroll 1
-          for (int u = 0; u < kWords; u += kStep) {
-            uint32_t w[kStep];
-            load_words<kStep>(value_codes + 4 * u, w);
+          for (int u = 0; u < kWords; ++u) {
+            const int to = part * kWords + u;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + 4 * u);
+            uint4 first, second;
+            if constexpr (kPSplit<HD>) {
+              two_parts(w, s2, low2, &first, &second);
+              *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, HD / 8 + to, kT)) = second;
+            } else {
+              uint32_t y[4];
 #pragma unroll
-            for (int k = 0; k < kStep; ++k) {
-              const int to = part * kWords + u + k;
-              uint4 first, second;
-              if constexpr (kPSplit<HD>) {
-                two_parts(w[k], s2, low2, &first, &second);
-                *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, HD / 8 + to, kT)) = second;
-              } else {
-                uint32_t y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t c = (w[k] >> (4 * j) & 0x000f000fu) | 0x64006400u;
-                  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c),
-                                            __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));  // code - 8
-                  y[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-                first = make_uint4(y[0], y[1], y[2], y[3]);
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t c = (w >> (4 * j) & 0x000f000fu) | 0x64006400u;
+                const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c),
+                                          __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));  // code - 8
+                y[j] = *reinterpret_cast<const uint32_t*>(&h);
               }
-              *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, to, kT)) = first;
+              first = make_uint4(y[0], y[1], y[2], y[3]);
             }
+            *reinterpret_cast<uint4*>(dst + unit_at<kPCols<HD>>(key, to, kT)) = first;
           }
         }
         fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&v_full[buf]);
+          mbar_arrive(v ? &v_full[buf] : &k_full[buf]);
           mbar_arrive(&raw_free[rs]);
         }
       }
       if (ok && g < run) at.next_item(a);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsRest));
-    if (warp == 12) {
+    if (warp == 16) {
       // ------------------------------------------------------------------ load
       const int bytes = kv4_head_bytes(sub_shift, HD);
       const auto page_of = [&]() {
@@ -733,83 +795,105 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       if (!ok)  // a wait ran out: leave once the copies in flight have landed
         for (int k = max(0, g - kPRaw); k < g; ++k)
           mbar_wait(&raw_full[k % kPRaw], static_cast<uint32_t>(k / kPRaw) & 1u, a.status);
-    } else if (warp == 13) {
+    } else if (warp == 17) {
       // ------------------------------------------------------------------- MMA
       constexpr uint32_t sw = HD == 32 ? 4 : 2, sbo = HD == 32 ? 512 : 1024;  // value rows: 128 bytes
       constexpr uint32_t idesc_s = idesc_f16_f32(kPBlock, kT);
-      constexpr uint32_t idesc_o = idesc_f16_f32(kPBlock, kPCols<HD>) | 1u << 16;  // B contiguous along N
+      constexpr uint32_t idesc_o = idesc_f16_f32(kPBlock, kPSums<HD>) | 1u << 16;  // B contiguous along N
       // operand descriptors of the first buffers; others lie at offsets in 16 bytes, which no field overflows on
-      const uint64_t q0 = operand_desc(smem_u32(sQ), 16, sbo, sw), k0 = operand_desc(smem_u32(sK), 16, sbo, sw);
-      const uint64_t qs0 = operand_desc(smem_u32(sS), 16, 256, 6);
-      const uint64_t ks0 = operand_desc(smem_u32(sK) + 2 * kPHalfBytes<HD>, 16, 256, 6);
-      const uint64_t v0 = operand_desc(smem_u32(sV), kT * 128, 1024, 2);
-      const auto scores = [&](int tile, int b, bool last) {
-        const uint64_t q = q0 + b * (kPQBytes<HD> / 32), k = k0 + (tile & 1) * (kPKeyBytes<HD> / 16);
+      // The whole warp runs this role and one elected lane issues: so addresses and descriptors stay in uniform registers,
+      // which the MMAs take them from.
+      const uint32_t tm = static_cast<uint32_t>(same(static_cast<int>(tmem)));
+      const uint32_t base = static_cast<uint32_t>(same(static_cast<int>(smem_u32(smem))));
+      constexpr uint32_t oS = kPQBytes<HD>, oK = oS + kPRows * 32, oV = oK + 2 * kPKeyBytes<HD>;
+      // operand descriptors of the first buffers; others lie at offsets in 16 bytes, which no field overflows on
+      const uint64_t q0 = operand_desc(base, 16, sbo, sw), k0 = operand_desc(base + oK, 16, sbo, sw);
+      const uint64_t qs0 = operand_desc(base + oS, 16, 256, 6);
+      const uint64_t ks0 = operand_desc(base + oK + 2 * kPHalfBytes<HD>, 16, 256, 6);
+      const uint64_t v0 = operand_desc(base + oV, kT * 128, 1024, 2);
+      // scores of block b and K buffer `buf` into a place of the ring
+      const auto scores = [&](int place, int buf, int b, bool last) {
+        const uint32_t at_key = static_cast<uint32_t>(buf * (kPKeyBytes<HD> / 16));
+        const uint64_t q = q0 + static_cast<uint32_t>(b * (kPQBytes<HD> / 32)), k = k0 + at_key;
+        const uint64_t qs = qs0 + static_cast<uint32_t>(b * (kPBlock * 2)), ks = ks0 + at_key;
+        const uint32_t to = tm + place * kT;
+        if (elect_one()) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < HD / 16; ++j)  // 16 values are 32 bytes
-            tc_mma_f16(tmem + b * 128, q + (j >> 2) * (kPBlock * 8) + (j & 3) * 2,
-                       k + h * (kPHalfBytes<HD> / 16) + (j >> 2) * (kT * 8) + (j & 3) * 2, idesc_s, (h | j) ? 1u : 0u);
-        tc_mma_f16(tmem + b * 128, qs0 + b * (kPBlock * 2), ks0 + (tile & 1) * (kPKeyBytes<HD> / 16), idesc_s, 1u);
-        tc_commit(&s_full[b]);
-        if (last) tc_commit(&k_free[tile & 1]);
-      };
-      int tiles[2] = {0, 0}, items[2] = {0, 0};  // of each block so far
-      bool ok = true;
-      while (g < run && ok) {
-        const int blocks = blocks_of(at), t1 = min(at.tiles, at.tile + run - g), end = g + t1 - at.tile;
-        if (lane == 0) {
-          ok = mbar_wait(&k_full[g & 1], static_cast<uint32_t>(g >> 1) & 1u, a.status);
-          for (int b = 0; b < blocks && ok; ++b) {
-            ok = mbar_wait(&q_full[b], static_cast<uint32_t>(items[b]) & 1u, a.status);
-            if (!ok) break;
-            tc_fence_after();
-            scores(g, b, b == blocks - 1);
-          }
-          bool fresh = true;
-          for (int i = g; i < end && ok; ++i) {
-            ok = mbar_wait(&v_full[i & 1], static_cast<uint32_t>(i >> 1) & 1u, a.status) &&
-                 (i + 1 == end || mbar_wait(&k_full[(i + 1) & 1], static_cast<uint32_t>((i + 1) >> 1) & 1u, a.status));
-            for (int b = 0; b < blocks && ok; ++b) {
-              const uint64_t v = v0 + (i & 1) * (kPValBytes<HD> / 16);
-              const uint32_t weights = tmem + b * 128, sums = weights + kO;
-              // the weights (the first half before the second), and for an item's first tile the sums' columns
-              if (fresh) ok = mbar_wait(&o_free[b], (static_cast<uint32_t>(items[b]) & 1u) ^ 1u, a.status);
-              if (kT == 128) {
-                ok = ok && mbar_wait(&p_half[b], static_cast<uint32_t>(tiles[b]) & 1u, a.status);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int j = 0; j < kT / 32; ++j)
-                  tc_mma_f16_ts(sums, weights + j * 8, v + j * 128, idesc_o, fresh && j == 0 ? 0u : 1u);
-              }
-              ok = ok && mbar_wait(&p_full[b], static_cast<uint32_t>(tiles[b]) & 1u, a.status);
-              if (!ok) break;
-              ++tiles[b];
-              tc_fence_after();
-#pragma unroll
-              for (int j = kT == 128 ? kT / 32 : 0; j < kT / 16; ++j)
-                tc_mma_f16_ts(sums, weights + j * 8, v + j * 128, idesc_o, fresh && j == 0 ? 0u : 1u);
-              if (b == blocks - 1) tc_commit(&v_free[i & 1]);
-              if (i + 1 < end) {
-                scores(i + 1, b, b == blocks - 1);  // over the weights just read: MMAs run in order
-              } else {
-                tc_commit(&o_full[b]);
-                ++items[b];
-              }
-            }
-            fresh = false;
-          }
+            for (int j = 0; j < HD / 16; ++j)  // 16 values are 32 bytes
+              tc_mma_f16(to, q + (j >> 2) * (kPBlock * 8) + (j & 3) * 2,
+                         k + h * (kPHalfBytes<HD> / 16) + (j >> 2) * (kT * 8) + (j & 3) * 2, idesc_s, (h | j) ? 1u : 0u);
+          tc_mma_f16(to, qs, ks, idesc_s, 1u);
+          tc_commit(&s_full[place]);
+          if (last) tc_commit(&k_free[buf]);
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();
+      };
+      // a step's weights times 16 keys j of its values
+      const auto product = [&](uint32_t sums, uint32_t weights, uint64_t v, int j, uint32_t accumulate) {
+        tc_mma_f16_ts(sums, weights + j * 8, v + j * 128, idesc_o, accumulate);
+        if constexpr (kPSplit<HD> && !kPSide<HD>) tc_mma_f16_ts(sums, weights + j * 8, v + kT * 8 + j * 128, idesc_o, 1u);
+      };
+      const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.status)) != 0;
+      };
+      int item = 0, item1 = 0;  // so far: all, and those of two blocks
+      int place = 0;  // the ring's turn of the item's next step, and the parity of its round
+      uint32_t round = 0;
+      bool ok = true;
+      g = 0;
+      const int n_run = same(run);
+      while (g < n_run && ok) {
+        const int blocks = same(blocks_of(at)), end = same(g + min(at.tiles, at.tile + n_run - g) - at.tile);
+        // Steps: the first block's tile, the second's, the next tile ...  The scores run ahead of the sums by the
+        // ring, one block's by two tiles (there are two buffers of K): a softmax group finds its next scores done.
+        const int lead = blocks == 2 ? kR : 2;
+        int next = g, next_b = 0, next_place = place;  // of the scores
+        const auto issue = [&]() {
+          if (next == end) return true;
+          if (next_b == 0 && !wait(&k_full[next & 1], static_cast<uint32_t>(next >> 1) & 1u)) return false;
+          if (next == g && !wait(&q_full[next_b], static_cast<uint32_t>(next_b ? item1 : item) & 1u)) return false;
+          tc_fence_after();
+          scores(next_place, next & 1, next_b, next_b == blocks - 1);
+          if (++next_place == kR) next_place = 0;
+          if (++next_b == blocks) next_b = 0, ++next;
+          return true;
+        };
+#pragma unroll 1
+        for (int k = 0; k < lead && ok; ++k) ok = issue();
+#pragma unroll 1
+        for (int i = g, b = 0; i < end && ok;) {
+          const uint64_t v = v0 + static_cast<uint32_t>((i & 1) * (kPValBytes<HD> / 16));
+          const uint32_t weights = tm + place * kT, sums = tm + kO + b * kPSums<HD>;
+          const uint32_t more = i > g;
+          // for an item's first tile the sums' columns; the values and the weights
+          ok = (more || wait(&o_free[b], (static_cast<uint32_t>(b ? item1 : item) & 1u) ^ 1u)) &&
+               __all_sync(0xffffffffu, wait_for(&v_full[i & 1], static_cast<uint32_t>(i >> 1) & 1u, &p_full[place], round,
+                                                a.status));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < kT / 16; ++j) product(sums, weights, v, j, j ? 1u : more);
+            tc_commit(&o_tile[b]);
+            if (i + 1 == end) tc_commit(&o_full[b]);
+            if (b == blocks - 1) tc_commit(&v_free[i & 1]);
+          }
+          __syncwarp();
+          if (++place == kR) place = 0, round ^= 1u;
+          ok = issue();  // over weights that have been read: MMAs run in order
+          if (++b == blocks) b = 0, ++i;
+        }
+        ++item;
+        if (blocks == 2) ++item1;
         g = end;
-        if (ok && g < run) at.next_item(a);
+        if (ok && g < n_run) at.next_item(a);
       }
     }
   }
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, kPTmemCols);
   }
@@ -822,12 +906,6 @@ int launch_prompt(const AttnArgs& a, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    cudaFuncAttributes at{};
-    if (int rc = check_cuda(cudaFuncGetAttributes(&at, kv4_prompt_kernel<HD>), "cudaFuncGetAttributes(kv4_prompt)"))
-      return rc;
-    // the roles' register shares come out of the launch's
-    if (at.numRegs * 4 < 2 * kPRegsSoftmax + kPRegsUnpack + kPRegsRest)
-      return fail(GSVK_ERR_UNSUPPORTED, "kv4_prompt_kernel: built with %d registers", at.numRegs);
     if (int rc = check_cuda(cudaFuncSetAttribute(kv4_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  kPSmem<HD>),
                             "cudaFuncSetAttribute(kv4_prompt)"))
