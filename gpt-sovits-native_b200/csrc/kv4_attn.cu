@@ -40,7 +40,14 @@ namespace {
 // maximum is one redux.
 constexpr int kTile = 64;          // keys of a unit
 constexpr int kSplitWarps = 4;     // warps of a CTA
-constexpr int kMaxPieces = 64;     // warps that share an item
+// Units that a warp takes at least of an item of `most`: with p pieces the warps take most / p units each and the join
+// p pieces, so the best p goes with the root; a unit takes about eight times a piece's part of the join of up to
+// four rows, four times that of sixteen.  One request of 4,000 keys, 8 heads of 64: 12 us (1 row), 16 (4 rows) and 39
+// (16); with up to 64 pieces whatever the length 14, 39 and 138, of 60,000 keys 39, 77 and 223 against 38, 48 and 110.
+template <int ROWS>
+__device__ __forceinline__ int least_share(int most) {
+  return static_cast<int>(sqrtf(static_cast<float>(most) * (ROWS >= 8 ? 0.25f : 0.125f)) + 0.5f);
+}
 
 template <int HD, int ROWS>
 constexpr int kCtasPerSm = HD == 128 ? 2 : (HD == 64 ? 3 : 4) - (ROWS == 16);
@@ -311,36 +318,56 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   }
 }
 
-// Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.
+// Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.  The
+// loads of up to four rows and four pieces are in flight together; row by row and two pieces at a time the join was most
+// of a short call's time (64 requests of 1,000 to 2,000 keys, 16 rows on 8 heads of 32: 58 us, 76 so).
 template <int HD, int ROWS>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Request& rq, int head, int block, int first, int last,
                                             int lane) {
-  constexpr int kD = HD / 32;
+  constexpr int kD = HD / 32, kSide = ROWS < 4 ? ROWS : 4, kAhead = kSide > 1 && HD == 128 ? 2 : 4;
   const int rows = min(ROWS, rq.n * a.group - block * ROWS), n = last - first + 1;
   const size_t stride = static_cast<size_t>(2) * ROWS * kRecord<HD>;  // from a warp's records to the next's
 #pragma unroll 1
-  for (int row = 0; row < rows; ++row) {
-    // the first warp's piece is its last one (second record), the others' their first
-    const float* r0 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + ROWS + row) * kRecord<HD>;
-    const float* r1 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + row) * kRecord<HD>;
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, (i ? r1 + i * stride : r0)[0]);
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[kD];
+  for (int row0 = 0; row0 < rows; row0 += kSide) {
+    // the first warp's piece is its last one (second record), the others' their first; rows past the last hold
+    // numbers of no meaning and are not written
+    const float* r0 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + ROWS + row0) * kRecord<HD>;
+    const float* r1 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + row0) * kRecord<HD>;
+    float base[kSide], sum[kSide], acc[kSide][kD];
 #pragma unroll
-    for (int d = 0; d < kD; ++d) acc[d] = 0.f;
-#pragma unroll 4
+    for (int k = 0; k < kSide; ++k) base[k] = -INFINITY;
+#pragma unroll 1
+    for (int i = lane; i < n; i += 32) {
+      const float* r = i ? r1 + i * stride : r0;
+#pragma unroll
+      for (int k = 0; k < kSide; ++k) base[k] = fmaxf(base[k], r[k * kRecord<HD>]);
+    }
+#pragma unroll
+    for (int k = 0; k < kSide; ++k) {
+      base[k] = warp_max(base[k]);
+      if (base[k] == -INFINITY) base[k] = 0.f;
+      sum[k] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kD; ++d) acc[k][d] = 0.f;
+    }
+#pragma unroll(kAhead)
     for (int i = 0; i < n; ++i) {
       const float* r = i ? r1 + i * stride : r0;
-      const float w = ex2(r[0] - base);
-      sum = fmaf(w, r[1], sum);
 #pragma unroll
-      for (int d = 0; d < kD; ++d) acc[d] = fmaf(w, r[4 + lane + 32 * d], acc[d]);
+      for (int k = 0; k < kSide; ++k, r += kRecord<HD>) {
+        const float w = ex2(r[0] - base[k]);
+        sum[k] = fmaf(w, r[1], sum[k]);
+#pragma unroll
+        for (int d = 0; d < kD; ++d) acc[k][d] = fmaf(w, r[4 + lane + 32 * d], acc[k][d]);
+      }
     }
-    uint16_t* o = out_row(a, rq, head, block * ROWS + row, HD);
 #pragma unroll
-    for (int d = 0; d < kD; ++d) o[lane + 32 * d] = f2h(sum == 0.f ? 0.f : acc[d] / sum);
+    for (int k = 0; k < kSide; ++k) {
+      if (row0 + k >= rows) break;
+      uint16_t* o = out_row(a, rq, head, block * ROWS + row0 + k, HD);
+#pragma unroll
+      for (int d = 0; d < kD; ++d) o[lane + 32 * d] = f2h(sum[k] == 0.f ? 0.f : acc[k][d] / sum[k]);
+    }
   }
 }
 
@@ -362,7 +389,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
 
   if (lane < kS) mbar_init(&bars[warp][lane], 1);
   fence_barrier_init();
-  L::template measure<kThreads>(a, runs, warps, kMaxPieces);
+  L::template measure<kThreads>(a, runs, warps, [](int most) { return least_share<ROWS>(most); });
   const long long total = runs.before[kThreads];
   const int me = static_cast<int>(blockIdx.x) * kSplitWarps + warp;
   const long long u0 = me * runs.share, u1 = min(total, u0 + runs.share);
@@ -531,12 +558,15 @@ int launch_split(const AttnArgs& a, cudaStream_t st) {
   return check_launch("kv4_attn_split_kernel");
 }
 
-// Query rows of a request to a kv head from which on 128-row tiles are used.
-constexpr int kMostSplitRows = 64;
+// Query rows of a request to a kv head past which 128-row tiles are used.  8 requests of 1,000 to 2,000 keys on 8 heads of
+// 32: 24 to 64 rows take 58 us here and 32 there, 64 requests 115 to 176 and 106; 16 rows 35 and 30, but 64 requests 58
+// and 102.
+constexpr int kMostSplitRows = 16;
 
 // The workspace: tickets of both kernels (zero between calls), then their records.
 size_t split_warps(size_t hd) {
-  return static_cast<size_t>(sm_count()) * kSplitWarps * (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
+  return static_cast<size_t>(sm_count()) * kSplitWarps *
+         (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
 }
 size_t tickets_bytes(size_t hd) { return (split_warps(hd) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
 // Offset of the records: after both kernels' tickets.

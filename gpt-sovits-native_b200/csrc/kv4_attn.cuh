@@ -118,9 +118,9 @@ struct Line {
     long long share;                // units of a run
     int most;                       // units of the longest item
   };
-  // Measures the line: an equal share for each worker, and no less than lets max_pieces of them cover the longest item.
-  template <int THREADS>
-  __device__ static __forceinline__ void measure(const AttnArgs& a, Runs<THREADS>& r, int workers, int max_pieces) {
+  // Measures the line: an equal share for each worker, and no less than least(units of the longest item).
+  template <int THREADS, class Least>
+  __device__ static __forceinline__ void measure(const AttnArgs& a, Runs<THREADS>& r, int workers, const Least& least) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int per = (a.n_seq + THREADS - 1) / THREADS;
     if (tid == 0) r.most = 0;
@@ -142,7 +142,7 @@ struct Line {
     r.before[tid + 1] = inc;
     if (tid == 0) r.before[0] = 0;
     if (tid == THREADS - 1)
-      r.share = max((inc + workers - 1) / workers, static_cast<long long>((r.most + max_pieces - 1) / max_pieces));
+      r.share = max((inc + workers - 1) / workers, static_cast<long long>(least(r.most)));
     __syncthreads();
   }
   // The place of unit u0 < the line's length (a whole warp).

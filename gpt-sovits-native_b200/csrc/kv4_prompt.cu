@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
   __shared__ typename L::template Runs<kPThreads> runs;
   const int tid = threadIdx.x, warp = same(tid >> 5), lane = tid & 31;
 
-  L::template measure<kPThreads>(a, runs, static_cast<int>(gridDim.x), kPMaxPieces);
+  L::template measure<kPThreads>(a, runs, static_cast<int>(gridDim.x),
+                                 [](int most) { return (most + kPMaxPieces - 1) / kPMaxPieces; });
   const int me = static_cast<int>(blockIdx.x);
   const long long u0 = me * runs.share, u1 = min(runs.before[kPThreads], u0 + runs.share);
   if (u0 >= u1) {  // the whole CTA
