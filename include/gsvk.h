@@ -753,13 +753,17 @@ int gsvk_kv4_read(const gsvk_kv4_cache* cache, const int64_t* slots, size_t n_to
  * first prefix_i keys seen by every row, as in the T2S prefill
  * (t2s_engine.cpp:881-1034).  out = softmax(scale q.k) . v over those keys,
  * zeros where there is none.  Scores, statistics and sums are fp32, the
- * result is rounded to fp16 once.  Keys past the limit are not read into the
+ * result is rounded to fp16 once; the weights go into the last product as fp16
+ * (22 bits for requests of up to 16 rows to a kv head), against values less
+ * their row's middle at head_dim 128, which moves the result by 2^-11 of the
+ * values at most.  Keys past the limit are not read into the
  * result, whatever their page holds; entries of block_table outside
  * [0, n_pages) count as keys past the limit.  Rows outside every
  * request are left as they are.  max_q: a bound on the longest request's rows, for
  * the choice of kernel (results hold for any value).
  * workspace: DEVICE, 256-byte aligned, gsvk_kv4_attention_workspace() bytes, zero before the
- * first call and left so; calls that may overlap need one each. */
+ * first call and left fit for the next (its tickets zero); calls that may overlap need one each.
+ * Its size depends on the GPU and head_dim, not on the lengths: 22 to 60 MB. */
 typedef struct {
   gsvk_kv4_cache cache;
   const uint16_t* q; size_t q_stride;     /* elements between rows, a multiple of 8 */
