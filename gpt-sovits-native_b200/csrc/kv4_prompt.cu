@@ -185,7 +185,8 @@ __device__ __forceinline__ float unit_above(float x, float* per_unit) {
 
 template <int HD>
 constexpr int kPRecord = HD + 4;  // floats of a row's piece: reference, sum, (pad); values.  Four of each row, then four of each ...
-constexpr int kPMaxPieces = 16;   // CTAs that share an item
+// CTAs that share an item at most: 100 rows over 30,000 keys, 2 heads of 64, take 65 us, with 6 97 and with 40 83.
+constexpr int kPMaxPieces = 16;
 
 template <int HD>
 using PromptLine = Line<kPRows, kPTile<HD>, true>;
