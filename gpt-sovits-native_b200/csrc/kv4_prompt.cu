@@ -63,6 +63,10 @@ template <int HD>
 constexpr int kPSums = kPSide<HD> ? 2 * HD : HD;  // and of the sums
 template <int HD>
 constexpr int kPRing = kPTile<HD> == 128 ? 3 : 4;  // tiles of scores in TMEM
+// What the weights of a chunk of keys may sum to before the reference moves.  At head_dim 128 they go in times the values'
+// step in their unit, which reaches four (unpack, below): either way no product passes 2^15, and fp16 holds it.
+template <int HD>
+constexpr float kPHigh = kPSplit<HD> ? 32768.f : 8192.f;
 constexpr int kPPar = 3;  // tiles of parameters: no more than of scores, so that no group lags by a round
 
 // What the softmax needs of a tile's keys.
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
           }
         };
         // The reference is the first tile's maximum.  It follows a tile late when a tile's sum has passed 2^8, or at once
-        // when that of a chunk passes 2^15: every weight stays in fp16's range with no maximum to take of each tile.
+        // when that of a chunk passes kPHigh: every weight stays in fp16's range with no maximum to take of each tile.
         float rescale = t.rescale;
         bool follow = i == t0 || __any_sync(0xffffffffu, tile_sum > 256.f || rescale != 1.f);
         float to = ref;
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
           }
           // a row that has seen nothing yet: weights without end for all that it sees, which sets its reference
           const bool none = ref == -INFINITY;
-          const float nbase = none ? 1.0e38f : -ref, high = none ? 0.f : 32768.f;
+          const float nbase = none ? 1.0e38f : -ref, high = none ? 0.f : kPHigh<HD>;
           const uint64_t nb = pair(nbase, nbase), sc = pair(score, score);
           follow = false;
 #pragma unroll 1

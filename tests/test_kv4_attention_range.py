@@ -1,0 +1,101 @@
+"""Attention over the paged 4-bit cache at the ends of its number ranges, against the formula in 64 bits: caches of one
+request, written as codes and parameters, so that every score and value is known."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+class Cache:
+    """A request's K and V rows: codes [2, length, hd], step and low [2, length], one kv head."""
+
+    def __init__(self, length, hd, page=64):
+        self.page, self.hd = page, hd
+        self.code = torch.zeros(2, length, hd, dtype=torch.uint8)
+        self.step, self.low = torch.zeros(2, 2, length, dtype=torch.float16)
+
+    def values(self):
+        k, v = (self.code.double() * self.step.double()[..., None] + self.low.double()[..., None]).cuda()
+        return k, v
+
+    def pages(self):
+        length, hd, page = self.code.shape[1], self.hd, self.page
+        n = -(-length // page)
+        par = torch.full((2, n * page, 2), float("nan"), dtype=torch.float16)  # rows past the length: NaN
+        par[:, :length, 0], par[:, :length, 1] = self.step, self.low
+        codes = torch.zeros(2, n * page, hd // 2, dtype=torch.uint8)
+        codes[:, :length] = self.code[..., 0::2] | (self.code[..., 1::2] << 4)
+        codes = codes.view(2, n, -1).transpose(0, 1)
+        par = par.view(2, n, -1).transpose(0, 1).contiguous().view(torch.uint8)
+        return torch.cat([codes.reshape(n, -1), par.reshape(n, -1)], 1).contiguous().cuda()
+
+
+def _attend(dev, cache, q, scale, workspace=None, copies=1):
+    """The rows of `copies` requests that share the cache's pages.  Where there are many, an item's tiles follow each other
+    in one run; a lone request is cut into pieces of a few tiles."""
+    (length, hd), rows, heads, i32 = cache.code.shape[1:], len(q), q.shape[1], dict(dtype=torch.int32, device="cuda")
+    c = dev.KV4Cache(cache.pages(), cache.page, 1, hd)
+    table = torch.arange(c.n_pages, **i32).repeat(copies, 1)
+    ws = workspace or dev.KV4Workspace(copies, rows * copies, heads, 1, hd)
+    q = q.repeat(copies, 1, 1)
+    out = c.attention(q, rows * torch.arange(copies + 1, **i32), torch.full((copies,), length, **i32), table, scale, rows, ws,
+                      out=torch.full_like(q, 77.0))
+    torch.cuda.synchronize()
+    assert dev.device_status() == 0
+    return out.double().view(copies, rows, heads, hd)
+
+
+def _exact(cache, q, scale, weight_bits):
+    """The result and its bound.  The output's rounding: 2^-11 of it.  The weights': 2^-weight_bits of the sum of the
+    products.  32-bit scores (a sum of head_dim terms of magnitude S in all), statistics and sums: 2^-18 (1 + S) of the
+    greatest value that the row sees."""
+    k, v = cache.values()
+    n, length = len(q), len(k)
+    seen = torch.arange(length, device="cuda") < (length - n + 1 + torch.arange(n, device="cuda"))[:, None]
+    q = q.double()
+    z = torch.einsum("thd,jd->htj", q, k) * scale
+    p = torch.softmax(z.masked_fill(~seen, float("-inf")), -1)
+    size = torch.einsum("thd,jd->htj", q.abs(), k.abs()).mul(abs(scale)).masked_fill(~seen, 0).amax(-1).t()
+    most = (v.abs().amax(-1) * seen).amax(-1)
+    out = torch.einsum("htj,jd->thd", p, v)
+    bound = (2.0 ** -11 * out.abs() + 2.0 ** -weight_bits * torch.einsum("htj,jd->thd", p, v.abs()) +
+             (2.0 ** -18 * (1 + size) * most[:, None])[..., None] + 2.0 ** -24)
+    return out, bound
+
+
+def _check(dev, cache, q, scale, weight_bits, copies=1, rows=slice(None)):
+    got = _attend(dev, cache, q, scale, copies=copies)
+    want, bound = _exact(cache, q, scale, weight_bits)
+    assert torch.isfinite(got[:, rows]).all()
+    off = ((got - want).abs() / bound)[:, rows]
+    assert (off <= 1).all(), float(off.max())
+
+
+def _bits(rows):
+    return 22 if rows <= 16 else 11
+
+
+def _octaves(cache, z):
+    """K rows of one value each, so that a query of ones has the scores z ln 2 (scale ln 2)."""
+    cache.step[0], cache.low[0] = 0, (z / cache.hd).half()
+
+
+LN2 = 0.6931471805599453
+
+
+@pytest.mark.parametrize("octaves", [9.0, 11.5, 12.9, 13.5, 14.0, 14.5, 14.9, 20.0])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("step", [1.0, 3.75, 7.5, 8.0])
+def test_large_steps_under_a_late_maximum(dev, hd, step, octaves):
+    """Values whose steps grow to four times the first tile's unit, with one late key far above the scores before it."""
+    gen = torch.Generator().manual_seed(5)
+    length, n = 400, 40
+    c = Cache(length, hd)
+    z = torch.zeros(length)
+    z[300] = octaves
+    _octaves(c, z)
+    c.code[1] = torch.randint(0, 16, (length, hd), generator=gen, dtype=torch.uint8)
+    c.step[1], c.low[1] = step, -7.5 * step
+    c.step[1, :128], c.low[1, :128] = 1.0, -7.5
+    _check(dev, c, torch.ones(n, 1, hd, dtype=torch.float16, device="cuda"), LN2, 11,
+           copies=300)
