@@ -26,8 +26,8 @@ __device__ __forceinline__ void load8(const float* p, float* f) {
 }
 
 // 8 codes of a row with scale s > 0.  x * (1 / s) is within 1e-4 of the quotient (below 128): further than that from a tie
-// it rounds like the quotient, else the division itself is made.  A sum with 1.5 2^23 is rounded to an
-// integer, to even, with the code as its low byte.
+// it rounds like the quotient, else the division itself is made, as for a scale so small that its inverse is infinite.  A
+// sum with 1.5 2^23 is rounded to an integer, to even, with the code as its low byte.
 __device__ __forceinline__ uint2 codes8(const float* x, float s, float per_s) {
   constexpr float kRound = 12582912.f;
   float c[8], far = 0.f;
@@ -37,7 +37,7 @@ __device__ __forceinline__ uint2 codes8(const float* x, float s, float per_s) {
     c[i] = q + kRound;
     far = fmaxf(far, fabsf(q - (c[i] - kRound)));
   }
-  if (!(far < 0.4998f)) {
+  if (!(far < 0.4998f) || per_s > 3.0e38f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = __fdiv_rn(x[i], s) + kRound;
   }
@@ -92,19 +92,17 @@ __global__ void __launch_bounds__(256)
   if (tid == 0) scale[r] = s;
   const bool some = s > 0.f;
   const float per_s = __frcp_rn(some ? s : 1.f);
-  // a scale so small that its inverse is not a number's takes divisions
-  const bool tiny = !(per_s <= 3.0e38f);
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
     const int i = k * THREADS + tid;
-    if (i < whole) *reinterpret_cast<uint2*>(qr + 8 * i) = some && !tiny ? codes8(kept[k], s, per_s) : make_uint2(0, 0);
+    if (i < whole) *reinterpret_cast<uint2*>(qr + 8 * i) = some ? codes8(kept[k], s, per_s) : make_uint2(0, 0);
   }
   for (int i = KEEP * THREADS + tid; i < whole; i += THREADS) {
     float f[8];
     load8(xr + 8 * i, f);
-    *reinterpret_cast<uint2*>(qr + 8 * i) = some && !tiny ? codes8(f, s, per_s) : make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(qr + 8 * i) = some ? codes8(f, s, per_s) : make_uint2(0, 0);
   }
-  for (int i = some && tiny ? tid : 8 * whole + tid; i < n; i += THREADS)
+  for (int i = 8 * whole + tid; i < n; i += THREADS)
     qr[i] = some ? static_cast<int8_t>(rintf(__fdiv_rn(as_f32(xr[i]), s))) : 0;
 }
 
