@@ -94,9 +94,15 @@ def _vector(t, dtype, n, what):
     raise ValueError(f"{what}: {n} contiguous values expected")
 
 
-def _row_stride(t):
-    """Elements between the rows of a 2-D tensor (one row: any)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _row_stride(t, what):
+    """Elements between the rows of a 2-D tensor (one row: any), which may not
+    overlap: to the C ABI the stride 0 of an expanded tensor means dense rows."""
+    if t.shape[0] < 2:
+        return t.shape[1]
+    ld = t.stride(0)
+    if ld < t.shape[1]:
+        raise ValueError(f"{what}: rows of {t.shape[1]} values, {ld} apart, overlap")
+    return ld
 
 
 def _rows(t, dtype, heads, head_dim, what):
@@ -333,13 +339,13 @@ def quantize_rows_i8(x, q=None, scale=None, stream=None):
         if q.shape != x.shape:
             raise ValueError(f"q: {(rows, n)} expected, got {tuple(q.shape)}")
         qp = _tensor(q, torch.int8, 2, "q")
-        ldq = _row_stride(q)
+        ldq = _row_stride(q, "q")
     if scale is None:
         scale = _kept(torch.empty(rows, dtype=torch.float32, device=x.device), stream)
         sp = scale.data_ptr()
     else:
         sp = _vector(scale, torch.float32, rows, "scale")
-    check(lib().gsvk_quantize_rows_i8(xp, dtype is torch.float32, rows, n, _row_stride(x), qp, ldq,
+    check(lib().gsvk_quantize_rows_i8(xp, dtype is torch.float32, rows, n, _row_stride(x, "x"), qp, ldq,
                                       sp, _stream_for(stream, x)))
     return q, scale
 
@@ -367,7 +373,7 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, residual=None, act=ACT_NONE, slop
         hp, ldh = c_f16.data_ptr(), N
     if residual is not None:
         rp, ldr = _matrix(residual, f32, M, N, "residual")
-    g = GemmI8Args(ap, a.stride(0) if M > 1 else K, bp, b.stride(0) if N > 1 else K,
+    g = GemmI8Args(ap, _row_stride(a, "a"), bp, _row_stride(b, "b"),
                    _vector(a_scale, f32, M, "a_scale"), _vector(b_scale, f32, N, "b_scale"), M, N, K,
                    None if bias is None else _vector(bias, f32, N, "bias"), rp, ldr, cp, ldc, hp,
                    ldh, act, slope)
@@ -380,4 +386,4 @@ def _matrix(t, dtype, M, N, what):
     p = _tensor(t, dtype, 2, what)
     if t.shape[0] != M or t.shape[1] != N:
         raise ValueError(f"{what}: {(M, N)} expected, got {tuple(t.shape)}")
-    return p, _row_stride(t)
+    return p, _row_stride(t, what)
