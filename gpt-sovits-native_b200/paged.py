@@ -121,10 +121,12 @@ class T2SPaged:
 
     def logits(self, x):
         """Logits (fp32) [max_seq, vocab] of each request's last row of a step;
-        those of a request that had none are of no meaning."""
+        those of a request that had none are of no meaning.  x: at least one row."""
         import torch
 
-        rows = x[(self.plan.q_start[1:] - 1).clamp(0, max(len(x) - 1, 0)).long()]
+        if len(x) == 0:  # the device would be asked for row 0 of none
+            raise ValueError("x: no rows, so no logits")
+        rows = x[(self.plan.q_start[1:] - 1).clamp(0, len(x) - 1).long()]
         return self.head(rows, c=torch.empty(self.max_seq, len(self.head.scale),
                                              dtype=torch.float32, device=self.device))
 
