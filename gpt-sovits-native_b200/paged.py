@@ -24,7 +24,8 @@ replayed.
 from __future__ import annotations
 
 from . import ACT_RELU, layernorm_rows
-from .quant import KV4Cache, KV4Workspace, KVPlan, gemm_i8, quantize_rows_i8
+from .quant import (KV4Cache, KV4Workspace, KVPlan, _row_stride, _tensor, _vector, gemm_i8,
+                    quantize_rows_i8)
 
 
 class Linear8:
@@ -103,11 +104,20 @@ class T2SPaged:
         self.plan.refused, keep their lengths and get rows of no meaning."""
         import torch
 
+        # all that a layer would refuse: the plan below moves the lengths on, so nothing may fail after it
+        _tensor(x, torch.float32, 2, "x")
+        _row_stride(x, "x")
+        if x.shape[1] != self.d_model:
+            raise ValueError(f"x: rows of {self.d_model} expected, got {x.shape[1]}")
         n = x.shape[0]
         if n > self.max_tokens:
             raise ValueError(f"x: {n} rows in a step of up to {self.max_tokens}")
+        if prefix is not None:
+            _vector(prefix, torch.int32, self.max_seq, "prefix")
         plan = self.plan.run(self.length, new_len, self.block_table, self.free_pages,
                              self.free_count, in_place=True)
+        if n == 0:  # every request rests
+            return x
         for layer in self.layers:
             qkv = layer["qkv"](x).view(n, 3, self.heads, self.head_dim)
             layer["cache"].append(qkv[:, 1], qkv[:, 2], plan.slots)
