@@ -117,10 +117,18 @@ def _rows(t, dtype, heads, head_dim, what):
     return p, row if n > 1 else heads * head_dim
 
 
-def _kept(t, stream):
-    """An output of this call, kept by the allocator until `stream` is done with it."""
-    if stream is not None:
-        t.record_stream(stream)
+def _empty(shape, dtype, device, stream):
+    """Memory for an output of this call.  For a call on another stream it is
+    that stream's (the current one's may still be in use by work that is
+    queued there), and the allocator keeps it until the current stream, whose
+    it is to read, is done with it too."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
     return t
 
 
@@ -268,9 +276,8 @@ class KV4Cache:
         n = slots.numel()
         sp = _vector(slots, torch.int64, n, "slots")
         if k is None and v is None:
-            k = _kept(torch.empty((n, self.kv_heads, self.head_dim), dtype=torch.float16,
-                                  device=slots.device), stream)
-            v = _kept(torch.empty_like(k), stream)
+            k, v = (_empty((n, self.kv_heads, self.head_dim), torch.float16, slots.device, stream)
+                    for _ in range(2))
         kp = ks = vp = vs = 0
         for t, what in ((k, "k"), (v, "v")):
             if t is not None and t.shape[0] != n:
@@ -298,7 +305,7 @@ class KV4Cache:
         a = self._attn
         a.q, a.q_stride = _rows(q, f16, heads, self.head_dim, "q")
         if out is None:
-            out = _kept(torch.empty((n, heads, self.head_dim), dtype=f16, device=q.device), stream)
+            out = _empty((n, heads, self.head_dim), f16, q.device, stream)
             a.out, a.out_stride = out.data_ptr(), heads * self.head_dim
         else:
             if out.shape != q.shape:
@@ -331,7 +338,7 @@ def quantize_rows_i8(x, q=None, scale=None, stream=None):
     rows, n = x.shape
     if q is None:
         ldq = (n + 15) & ~15
-        q = _kept(torch.empty((rows, ldq), dtype=torch.int8, device=x.device), stream)
+        q = _empty((rows, ldq), torch.int8, x.device, stream)
         qp = q.data_ptr()
         if ldq != n:
             q = q[:, :n]
@@ -341,7 +348,7 @@ def quantize_rows_i8(x, q=None, scale=None, stream=None):
         qp = _tensor(q, torch.int8, 2, "q")
         ldq = _row_stride(q, "q")
     if scale is None:
-        scale = _kept(torch.empty(rows, dtype=torch.float32, device=x.device), stream)
+        scale = _empty(rows, torch.float32, x.device, stream)
         sp = scale.data_ptr()
     else:
         sp = _vector(scale, torch.float32, rows, "scale")
@@ -369,7 +376,7 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, residual=None, act=ACT_NONE, slop
     if c_f16 is not None:
         hp, ldh = _matrix(c_f16, torch.float16, M, N, "c_f16")
     elif c is None:
-        c_f16 = _kept(torch.empty((M, N), dtype=torch.float16, device=a.device), stream)
+        c_f16 = _empty((M, N), torch.float16, a.device, stream)
         hp, ldh = c_f16.data_ptr(), N
     if residual is not None:
         rp, ldr = _matrix(residual, f32, M, N, "residual")

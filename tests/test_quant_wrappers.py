@@ -1,4 +1,7 @@
 """What the Python calls of the quantised operators refuse before anything is launched, and whose memory they use."""
+import contextlib
+import types
+
 import pytest
 import torch
 
@@ -30,3 +33,52 @@ def test_expanded_tensors_are_refused(dev):
             call()
     # one row has no stride
     assert dev.gemm_i8(a[:1].expand(1, 64), s, a, s, residual=x[:4].expand(1, 4)).shape == (1, 4)
+
+
+def test_outputs_on_another_stream_are_its_memory(gsv, monkeypatch):
+    """The allocator is asked from within the call's stream, and told of the one that reads the result."""
+    from gsv_b200 import quant
+
+    asked, told, inside = [], [], []
+
+    @contextlib.contextmanager
+    def use(stream):
+        inside.append(stream)
+        yield
+        inside.pop()
+
+    def empty(shape, **kw):
+        asked.append(inside[-1] if inside else "current")
+        return types.SimpleNamespace(record_stream=told.append)
+
+    monkeypatch.setattr(torch.cuda, "stream", use)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: inside[-1] if inside else "current")
+    monkeypatch.setattr(torch, "empty", empty)
+    quant._empty((2, 3), torch.float16, "cuda:0", None)
+    quant._empty((2, 3), torch.float16, "cuda:0", "other")
+    assert asked == ["current", "other"] and told == ["current"]
+
+
+@pytest.mark.gpu
+def test_outputs_on_another_stream_are_not_the_current_ones_memory(dev):
+    """Blocks that the current stream has given back may still be written by its queued work: a call on another stream gets
+    none of them."""
+    other = torch.cuda.Stream()
+    x = torch.randn(2048, 1024, device="cuda").half()
+    w, ws = dev.quantize_rows_i8(x)
+    c = dev.KV4Cache.empty(8, 64, 4, 128)
+    slots = torch.arange(512, device="cuda")
+    c.append(x.view(-1, 4, 128)[:512], x.view(-1, 4, 128)[:512], slots)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, space = torch.arange(8, dtype=torch.int32, device="cuda")[None], dev.KV4Workspace(1, 512, 4, 4, 128)
+    rows, q_start, kv_len = x.view(-1, 4, 128)[:512], i32(0, 512), i32(512)
+    calls = (lambda s: dev.quantize_rows_i8(x, stream=s), lambda s: [dev.gemm_i8(w, ws, w, ws, stream=s)],
+             lambda s: c.read(slots, stream=s),
+             lambda s: [c.attention(rows, q_start, kv_len, table, 0.1, 512, space, stream=s)])
+    torch.cuda.synchronize()
+    for call in calls:
+        given_back = {t.data_ptr() for t in call(None)}
+        torch.cuda.synchronize()
+        out = call(other)
+        other.synchronize()
+        assert not given_back & {t.data_ptr() for t in out}
