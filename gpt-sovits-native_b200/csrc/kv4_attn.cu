@@ -577,14 +577,16 @@ int launch_split(const AttnArgs& a, cudaStream_t st) {
 // and 102.
 constexpr int kMostSplitRows = 16;
 
-// The workspace: tickets of both kernels (zero between calls), then their records.
+// The workspace: tickets of both kernels (zero between calls), then their records.  The tickets' places are those of the
+// most warps whatever the head_dim, so that calls of every head_dim can share a workspace: no record lies on a ticket.
 size_t split_warps(size_t hd) {
   return static_cast<size_t>(sm_count()) * kSplitWarps *
          (hd == 128 ? kCtasPerSm<128, 1> : hd == 64 ? kCtasPerSm<64, 1> : kCtasPerSm<32, 1>);
 }
-size_t tickets_bytes(size_t hd) { return (split_warps(hd) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
+static_assert(kCtasPerSm<32, 1> >= kCtasPerSm<64, 1> && kCtasPerSm<32, 1> >= kCtasPerSm<128, 1>);
+size_t tickets_bytes() { return (split_warps(32) * sizeof(int) + 255) & ~static_cast<size_t>(255); }
 // Offset of the records: after both kernels' tickets.
-size_t attention_parts(size_t hd) { return tickets_bytes(hd) + kv4_prompt_ticket_bytes(); }
+size_t attention_parts() { return tickets_bytes() + kv4_prompt_ticket_bytes(); }
 // Whether some request of n_tokens rows may have enough for the kernel for longer requests.
 bool may_be_long(size_t n_tokens, size_t group) { return n_tokens * group > kMostSplitRows; }
 
@@ -601,7 +603,7 @@ size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads,
       heads == 0 || heads > 65536 || n_tokens > 0x7fffffff / (heads / kv_heads) ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return 0;
-  return attention_parts(head_dim) + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float) +
+  return attention_parts() + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float) +
          (may_be_long(n_tokens, heads / kv_heads) ? kv4_prompt_part_bytes(head_dim) : 0);
 }
 
@@ -652,9 +654,9 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   a.scale_log2 = g->scale * 1.4426950408889634f;
   a.tickets = static_cast<int*>(g->workspace);
   uint8_t* ws = static_cast<uint8_t*>(g->workspace);
-  a.long_tickets = reinterpret_cast<int*>(ws + tickets_bytes(hd));
-  a.parts = reinterpret_cast<float*>(ws + attention_parts(hd));
-  a.long_parts = reinterpret_cast<float*>(ws + attention_parts(hd) + split_warps(hd) * 2 * 16 * (hd + 4) * sizeof(float));
+  a.long_tickets = reinterpret_cast<int*>(ws + tickets_bytes());
+  a.parts = reinterpret_cast<float*>(ws + attention_parts());
+  a.long_parts = reinterpret_cast<float*>(ws + attention_parts() + split_warps(hd) * 2 * 16 * (hd + 4) * sizeof(float));
   a.status = device_status();
   cudaStream_t st = as_cuda(stream);
   // Requests with more rows than this take the kernel with 128-row tiles.

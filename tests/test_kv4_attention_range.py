@@ -99,3 +99,26 @@ def test_large_steps_under_a_late_maximum(dev, hd, step, octaves):
     c.step[1, :128], c.low[1, :128] = 1.0, -7.5
     _check(dev, c, torch.ones(n, 1, hd, dtype=torch.float16, device="cuda"), LN2, 11,
            copies=300)
+
+
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_calls_of_every_head_dim_share_a_workspace(dev, hd, rows):
+    """What a call of head_dim 128 leaves in the records is no ticket of another head_dim's: items that several warps or
+    CTAs share are joined as on a workspace of their own."""
+    gen = torch.Generator().manual_seed(8)
+
+    def cache(d, length):
+        c = Cache(length, d)
+        c.code[:] = torch.randint(0, 16, c.code.shape, generator=gen, dtype=torch.uint8)
+        c.step[:], c.low[:] = 0.1, -0.75
+        return c
+
+    big, small = cache(128, 3000), cache(hd, 9000)
+    qb, qs = (torch.randn(n, 1, d, generator=gen).half().cuda() for n, d in ((1, 128), (rows, hd)))
+    ws = dev.KV4Workspace(40, 40 * 300, 1, 1, 128)
+    alone = _attend(dev, small, qs, 0.1, copies=40)
+    assert not (alone == 77).any()
+    for _ in range(2):
+        _attend(dev, big, qb, 0.1, ws, copies=40)
+        assert torch.equal(_attend(dev, small, qs, 0.1, ws, copies=40), alone)
