@@ -24,8 +24,8 @@ replayed.
 from __future__ import annotations
 
 from . import ACT_RELU, layernorm_rows
-from .quant import (KV4Cache, KV4Workspace, KVPlan, _row_stride, _tensor, _vector, gemm_i8,
-                    quantize_rows_i8)
+from .quant import (KV4Cache, KV4Workspace, KVPlan, _device, _device_for, _row_stride, _tensor,
+                    _vector, gemm_i8, quantize_rows_i8)
 
 
 class Linear8:
@@ -50,7 +50,7 @@ class T2SPaged:
         import numpy as np
         import torch
 
-        device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+        device = _device_for(device)
         self.device, self.max_seq, self.max_tokens = device, int(max_seq), int(max_tokens)
         self.d_model, self.heads = model["d_model"], model["n_heads"]
         self.head_dim = self.d_model // self.heads
@@ -105,15 +105,16 @@ class T2SPaged:
         import torch
 
         # all that a layer would refuse: the plan below moves the lengths on, so nothing may fail after it
-        _tensor(x, torch.float32, 2, "x")
-        _row_stride(x, "x")
+        here = _device()
+        _tensor(x, torch.float32, 2, "x", here)
+        _row_stride(x, *x.shape, "x")
         if x.shape[1] != self.d_model:
             raise ValueError(f"x: rows of {self.d_model} expected, got {x.shape[1]}")
         n = x.shape[0]
         if n > self.max_tokens:
             raise ValueError(f"x: {n} rows in a step of up to {self.max_tokens}")
         if prefix is not None:
-            _vector(prefix, torch.int32, self.max_seq, "prefix")
+            _vector(prefix, torch.int32, self.max_seq, "prefix", here)
         plan = self.plan.run(self.length, new_len, self.block_table, self.free_pages,
                              self.free_count, in_place=True)
         if n == 0:  # every request rests

@@ -9,11 +9,11 @@ import torch
 def test_rows_that_overlap_have_no_stride(gsv):
     from gsv_b200 import quant
 
-    assert quant._row_stride(torch.zeros(1, 8).expand(1, 8), "x") == 8
-    assert quant._row_stride(torch.zeros(4, 12)[:, :8], "x") == 12
+    assert quant._row_stride(torch.zeros(1, 8).expand(1, 8), 1, 8, "x") == 8
+    assert quant._row_stride(torch.zeros(4, 12)[:, :8], 4, 8, "x") == 12
     for t in (torch.zeros(8).expand(4, 8), torch.zeros(40).as_strided((4, 8), (7, 1))):
         with pytest.raises(ValueError, match="overlap"):
-            quant._row_stride(t, "x")
+            quant._row_stride(t, 4, 8, "x")
 
 
 @pytest.mark.gpu
@@ -54,8 +54,8 @@ def test_outputs_on_another_stream_are_its_memory(gsv, monkeypatch):
     monkeypatch.setattr(torch.cuda, "stream", use)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: inside[-1] if inside else "current")
     monkeypatch.setattr(torch, "empty", empty)
-    quant._empty((2, 3), torch.float16, "cuda:0", None)
-    quant._empty((2, 3), torch.float16, "cuda:0", "other")
+    for stream in (None, "other"):
+        quant._allocator(stream)((2, 3), dtype=torch.float16, device="cuda:0")
     assert asked == ["current", "other"] and told == ["current"]
 
 
@@ -82,3 +82,61 @@ def test_outputs_on_another_stream_are_not_the_current_ones_memory(dev):
         out = call(other)
         other.synchronize()
         assert not given_back & {t.data_ptr() for t in out}
+
+
+def _foreign(index):
+    """What the checks ask of a contiguous fp32 tensor [4, 8] on a device."""
+    return types.SimpleNamespace(dtype=torch.float32, is_cuda=True, shape=(4, 8), dim=lambda: 2, stride=lambda i: (8, 1)[i],
+                                 is_contiguous=lambda: True, numel=lambda: 32, data_ptr=lambda: 256, get_device=lambda: index)
+
+
+def test_tensors_streams_and_buffers_of_another_device_are_refused(gsv, monkeypatch):
+    from gsv_b200 import quant
+
+    for f in (lambda t: quant._tensor(t, torch.float32, 2, "x", 0), lambda t: quant._vector(t, torch.float32, 32, "x", 0)):
+        assert f(_foreign(0)) == 256
+        with pytest.raises(ValueError, match="cuda:1"):
+            f(_foreign(1))
+    stream = types.SimpleNamespace(cuda_stream=77, device_index=1)
+    assert quant._stream_for(stream, 1) == 77
+    with pytest.raises(ValueError, match="cuda:1"):
+        quant._stream_for(stream, 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    for make in (lambda d: gsv.KVPlan(2, 4, 16, 8, 8, device=d), lambda d: gsv.KV4Workspace(2, 2, 2, 2, 32, device=d),
+                 lambda d: gsv.KV4Cache.empty(2, 16, 2, 32, device=d)):
+        for device in ("cuda:1", torch.device("cuda", 1), "cpu"):
+            with pytest.raises(ValueError, match="current device"):
+                make(device)
+
+
+@pytest.mark.gpu
+def test_calls_run_where_the_current_device_is(dev, monkeypatch):
+    """With another device current, every call refuses this one's tensors; given as the current one, a device is taken."""
+    from gsv_b200 import quant
+
+    x = torch.randn(4, 64, device="cuda")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, s = dev.quantize_rows_i8(x)
+    for device in (None, "cuda", "cuda:0", torch.device("cuda", 0)):
+        c, ws = dev.KV4Cache.empty(4, 16, 2, 32, device=device), dev.KV4Workspace(1, 4, 2, 2, 32, device=device)
+        p = dev.KVPlan(1, 4, 16, 4, 4, device=device)
+    rows, slots, table = x.view(4, 2, 32).half(), torch.arange(4, device="cuda"), i32(0, 1, 2, 3)[None]
+    plan = (i32(0), i32(4), table, i32(0, 1, 2, 3), i32(4))
+    calls = (lambda: dev.quantize_rows_i8(x), lambda: dev.gemm_i8(q, s, q, s), lambda: c.append(rows, rows, slots),
+             lambda: c.read(slots), lambda: c.attention(rows, i32(0, 4), i32(4), table, 0.1, 4, ws), lambda: p.run(*plan),
+             lambda: p.release(i32(1), *plan[0:1], *plan[2:]))
+    for call in calls:
+        call()
+    monkeypatch.setattr(quant, "_device", lambda: 1)
+    for call in calls:
+        with pytest.raises(ValueError, match="cuda:0"):
+            call()
+    monkeypatch.undo()
+    ws.index = 1
+    with pytest.raises(ValueError, match="workspace"):
+        calls[4]()
+    for held, at in ((c, (2, 3, 4)), (p, (5, 6))):  # memory of another device behind arguments of this one
+        held._index = 1
+        for i in at:
+            with pytest.raises(ValueError, match="cuda:1"):
+                calls[i]()
