@@ -34,9 +34,12 @@ namespace {
 // rounded, and over 60,000 keys sums of positive codes moved the result by 1.6e-3 of
 // its size, at 135 us for 8 rows of 32 heads of 128 over as many keys each (2.1e-4 and
 // 156 us so, the rounding of the result; a sum of its own for each tile, 4e-4 and 151 us).
-// The weights p_j a_j, scaled by a power of two so that the greatest step seen is
-// at most 1, go in as two fp16 parts, whose sum holds 22 bits: up to 8 rows, the
-// second part takes the unused rows 8..15 of the same MMA.
+// The weights p_j a_j, scaled by a power of two so that the greatest step seen
+// comes to less than 2^15 (kTop), go in as two fp16 parts.  Their sum holds 22
+// bits of every weight down to 2^-17 of that bound, and all of them to
+// within 2^-40 of it: so 60,000 keys that each weigh 2^-25 of a first strong one
+// count in full (with weights up to 1 they were lost, 2^-9 of the values).  Up to
+// 8 rows, the second part takes the unused rows 8..15 of the same MMA.
 //
 // Between the products the scores pass through shared memory to a layout with
 // two keys to a lane, so that the softmax costs what the rows there are cost
@@ -52,6 +55,8 @@ template <int ROWS>
 __device__ __forceinline__ int least_share(int most) {
   return static_cast<int>(sqrtf(static_cast<float>(most) * (ROWS >= 8 ? 0.25f : 0.125f)) + 0.5f);
 }
+
+constexpr float kTop = 32768.f;  // what the weights' unit comes to as an operand: fp16's range ends at 65,504
 
 // As many CTAs as registers and shared memory take; with one less an SM the long caches' 156 us were 40 % longer.
 template <int HD, int ROWS>
@@ -232,11 +237,12 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   const float per_unit = unit > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(unit)) : 0.f;  // 1 / unit
   const float rescale = s.unit * per_unit;
   s.unit = unit;
+  const float scale_up = per_unit * kTop;
   const float a0 = h2f(static_cast<uint16_t>(kp0)) * (scale_log2 * 16777216.f), b0 = h2f(static_cast<uint16_t>(kp0 >> 16));
   const float a1 = h2f(static_cast<uint16_t>(kp1)) * (scale_log2 * 16777216.f), b1 = h2f(static_cast<uint16_t>(kp1 >> 16));
   const float step0 = h2f(static_cast<uint16_t>(vp0)), step1 = h2f(static_cast<uint16_t>(vp1));
-  const float st0 = step0 * per_unit, low0 = fmaf(8.f, step0, h2f(static_cast<uint16_t>(vp0 >> 16)));  // of code 8
-  const float st1 = step1 * per_unit, low1 = fmaf(8.f, step1, h2f(static_cast<uint16_t>(vp1 >> 16)));
+  const float st0 = step0 * scale_up, low0 = fmaf(8.f, step0, h2f(static_cast<uint16_t>(vp0 >> 16)));  // of code 8
+  const float st1 = step1 * scale_up, low1 = fmaf(8.f, step1, h2f(static_cast<uint16_t>(vp1 >> 16)));
   const int place = 8 * (g >> 1) + 2 * t + (g & 1);
   __syncwarp();
   float fix[kR];
@@ -491,7 +497,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
     // the warps that share the item
     const int first = me - (item_start < 0 ? (share - 1 - item_start) / share : 0);
     const int last = me + (item_start + at.tiles - 1) / share;
-    const float up = s.unit;
+    const float up = s.unit * (1.f / kTop);
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
       float l = 0.f, pb = 0.f, m = 0.f;

@@ -122,3 +122,45 @@ def test_calls_of_every_head_dim_share_a_workspace(dev, hd, rows):
     for _ in range(2):
         _attend(dev, big, qb, 0.1, ws, copies=40)
         assert torch.equal(_attend(dev, small, qs, 0.1, ws, copies=40), alone)
+
+
+def _strong_key(dev, hd, rows, drop, copies):
+    """60,000 keys `drop` octaves below the first: each weighs little, together they are most of the result, whose first
+    value is 0."""
+    length = 60000
+    c = Cache(length, hd)
+    z = torch.full((length,), -drop)
+    z[0] = 0
+    _octaves(c, z)
+    c.code[1], c.step[1], c.low[1] = 15, 0.125, -1.0  # 0.875, in a row that is centred on 0
+    c.code[1, 0] = 8  # 0
+    _check(dev, c, torch.ones(rows, 1, hd, dtype=torch.float16, device="cuda"), LN2, _bits(rows), copies)
+
+
+@pytest.mark.parametrize("drop", [12.0, 18.0, 21.0, 23.4, 25.0])
+@pytest.mark.parametrize("rows,copies", [(1, 3000), (4, 3000), (7, 1600), (16, 1600)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_one_strong_key_before_a_long_cache(dev, hd, rows, copies, drop):
+    _strong_key(dev, hd, rows, drop, copies)
+
+
+@pytest.mark.parametrize("rows", [4, 16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("size", [30.0, 3e3, 6e4])
+@pytest.mark.parametrize("part", [0, 1])
+def test_a_large_row_moves_none_that_does_not_see_it(dev, hd, rows, size, part):
+    _large_row(dev, hd, rows, size, part)
+
+
+def _large_row(dev, hd, rows, size, part):
+    """The last token's K (part 0) or V is far larger than all others: only the last row sees it."""
+    gen = torch.Generator().manual_seed(7)
+    length = 300
+    c = Cache(length, hd)
+    x = torch.randn(2, length, hd, generator=gen)
+    x[part, -1] = torch.randn(hd, generator=gen).sign() * size
+    lo, hi = x.amin(-1), x.amax(-1)
+    c.low[:], c.step[:] = lo.half(), ((hi - lo) / 15).half()
+    c.code[:] = ((x - c.low.float()[..., None]) / c.step.float()[..., None]).round().clamp(0, 15).to(torch.uint8)
+    q = torch.randn(rows, 1, hd, generator=gen).half().cuda()
+    _check(dev, c, q, hd ** -0.5, _bits(rows), copies=300, rows=slice(0, rows - 1))
