@@ -25,9 +25,11 @@
 // there, with the codes e - 8 as the operand and the last sum in the softmax.
 // Either way the one rounding to fp16 beside the result's is that of the
 // weights: 2^-11 of the values (centred within 8 steps at head_dim 128).
-// p_j = 2^(z_j - reference).  The reference is the maximum of the item's first tile, and moves only when a sum of
-// weights shows that they outgrow fp16's range: so the maximum is taken once an item and the sums in TMEM are
-// mostly left alone.  K and V (s) are divided by a power of two, that of K by tile, that of V the same for all rows.
+// p_j = 2^(z_j - reference).  The reference is six octaves (kPHead) below the maximum of the item's first tile, and moves
+// only when a sum of weights shows that they outgrow fp16's range: so the maximum is taken once an item and the sums in
+// TMEM are mostly left alone.  A weight is lost below 2^-31 of that maximum's: 60,000 keys that each weigh 2^-25 of a
+// first strong one count (with the reference at the maximum they did not, 2^-9 of the values).  K and V (s) are divided by
+// a power of two, that of K by tile, that of V the same for all rows.
 //
 // What bounds it, per 256 x 128 scores at head_dim 64: 2 x (9 + 16) MMAs of 67 clocks = 3,350, and 32,768
 // exponentials at 16 a clock = 2,048; a softmax warp takes 3,100 clocks for its 32 x 128 and some 7,000 between
@@ -63,6 +65,10 @@ template <int HD>
 constexpr int kPSums = kPSide<HD> ? 2 * HD : HD;  // and of the sums
 template <int HD>
 constexpr int kPRing = kPTile<HD> == 128 ? 3 : 4;  // tiles of scores in TMEM
+constexpr float kPHead = 6.f;  // octaves from the reference to the greatest score that sets it
+// A tile's sum of weights past which the reference follows: twice what scores that stay make at most.
+template <int HD>
+constexpr float kPFollow = 2.f * 64.f * kPTile<HD>;
 // What the weights of a chunk of keys may sum to before the reference moves.  At head_dim 128 they go in times the values'
 // step in their unit, which reaches four (unpack, below): either way no product passes 2^15, and fp16 holds it.
 template <int HD>
@@ -400,29 +406,31 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
             hide(c + 16, r + 16);
           }
         };
-        // The reference is the first tile's maximum.  It follows a tile late when a tile's sum has passed 2^8, or at once
-        // when that of a chunk passes kPHigh: every weight stays in fp16's range with no maximum to take of each tile.
+        // The reference is set by the first tile's maximum.  It follows a tile late when a tile's sum has passed kPFollow, or
+        // at once when that of a chunk passes kPHigh: every weight stays in fp16's range with no maximum to take of each tile.
         float rescale = t.rescale;
-        bool follow = i == t0 || __any_sync(0xffffffffu, tile_sum > 256.f || rescale != 1.f);
+        bool follow = i == t0 || __any_sync(0xffffffffu, tile_sum > kPFollow<HD> || rescale != 1.f);
         float to = ref;
-        if (tile_sum > 256.f) to += static_cast<float>(static_cast<int>(__float_as_uint(tile_sum) >> 23) - 127);
+        if (tile_sum > kPFollow<HD>) to += static_cast<float>(static_cast<int>(__float_as_uint(tile_sum) >> 23) - 127) - kPHead;
         tile_sum = 0.f;
         int c = 0;
         bool at_once = i == t0;
         for (;;) {
           if (follow) {
             if (at_once) {  // the maximum of what is left of the tile
+              float top = -INFINITY;
 #pragma unroll 1
               for (int k = c; k < kT; k += kChunk) {
                 uint32_t r[kChunk];
                 fetch(k, r);
-                float x[4] = {to, -INFINITY, -INFINITY, -INFINITY};
+                float x[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int j = 0; j < kChunk; j += 2)
                   x[(j >> 1) & 3] = fmaxf(fmaxf(x[(j >> 1) & 3], __uint_as_float(r[j]) * score),
                                           __uint_as_float(r[j + 1]) * score);
-                to = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
               }
+              to = fmaxf(to, top - kPHead);
             }
             if (i == t0) {
               ref = to;

@@ -164,3 +164,10 @@ def _large_row(dev, hd, rows, size, part):
     c.code[:] = ((x - c.low.float()[..., None]) / c.step.float()[..., None]).round().clamp(0, 15).to(torch.uint8)
     q = torch.randn(rows, 1, hd, generator=gen).half().cuda()
     _check(dev, c, q, hd ** -0.5, _bits(rows), copies=300, rows=slice(0, rows - 1))
+
+
+@pytest.mark.parametrize("drop", [12.0, 18.0, 21.0, 23.4, 25.0])
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_one_strong_key_before_a_long_cache_of_a_prompt(dev, hd, rows, drop):
+    _strong_key(dev, hd, rows, drop, 200)
