@@ -18,8 +18,8 @@
 // Mathematics.  k_j = a c + b (step, codes, low), so q.k_j = q.(a c) + sum(q) b.
 // a c takes 15 bits: it goes in as the sum of two fp16 numbers, one product
 // and one fused product for two codes, and b as one more column of K against
-// sum(q), which is two columns of Q.  So no score is rounded below fp32
-// (K as one fp16 number would move each by 2^-12 |q||k|).
+// sum(q), which is two columns of Q, 22 bits of it.  So a score is within
+// 2^-22 |q||k| of the exact one (K as one fp16 number would move it by 2^-12).
 // v_j goes in as two fp16 parts at head_dim 32 and 64.  At head_dim 128 that would double the MMAs:
 //   sum_j p_j v_j = sum_j (p_j s_j) (e_j - 8) + sum_j p_j (f_j + 8 s_j)
 // there, with the codes e - 8 as the operand and the last sum in the softmax.
@@ -29,7 +29,9 @@
 // only when a sum of weights shows that they outgrow fp16's range: so the maximum is taken once an item and the sums in
 // TMEM are mostly left alone.  A weight is lost below 2^-31 of that maximum's: 60,000 keys that each weigh 2^-25 of a
 // first strong one count (with the reference at the maximum they did not, 2^-9 of the values).  K and V (s) are divided by
-// a power of two, that of K by tile, that of V the same for all rows.
+// a power of two, that of K by tile, that of V the same for all rows.  The greatest then lies far up in fp16's range
+// (kPKeyTop, kPValTop), which leaves bits to the others: none is off by more than 2^-28 (K) or 2^-32 (V) of it.  So a row's
+// result does not hang on a key of 6e4 in its tile that it does not see (with the greatest at 1, 2^-20 of 6e4 were lost).
 //
 // What bounds it, per 256 x 128 scores at head_dim 64: 2 x (9 + 16) MMAs of 67 clocks = 3,350, and 32,768
 // exponentials at 16 a clock = 2,048; a softmax warp takes 3,100 clocks for its 32 x 128 and some 7,000 between
@@ -65,6 +67,9 @@ template <int HD>
 constexpr int kPSums = kPSide<HD> ? 2 * HD : HD;  // and of the sums
 template <int HD>
 constexpr int kPRing = kPTile<HD> == 128 ? 3 : 4;  // tiles of scores in TMEM
+// What the units of keys and values come to as operands, below 65,504 each: 128 b is a column of K, and a value may be four
+// times its unit, as the sum of two parts of that size.
+constexpr float kPKeyTop = 256.f, kPValTop = 4096.f;
 constexpr float kPHead = 6.f;  // octaves from the reference to the greatest score that sets it
 // A tile's sum of weights past which the reference follows: twice what scores that stay make at most.
 template <int HD>
@@ -686,7 +691,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         const float most = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
         TileParams<HD>& t = par[g % kPPar];
         if (!v) {
-          const float key_unit = unit_above(most, &per_unit);
+          const float key_unit = unit_above(most, &per_unit) * (1.f / kPKeyTop);
+          per_unit *= kPKeyTop;
           if (me_key == 0) {
             t.score = fmaxf(fabsf(a.scale_log2) * key_unit, 1e-30f);  // not 0, which a hidden score could not be scaled by
             t.page_ok = page_ok;
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
             }
           }
           if (me_key == 0) {
-            t.unit = unit;
+            t.unit = kPSplit<HD> ? unit * (1.f / kPValTop) : unit;
             t.rescale = rescale;
           }
           __syncwarp();
@@ -733,7 +739,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           uint8_t* dst = sV + buf * kPValBytes<HD>;
-          const __half2 s2 = __float2half2_rn(step * per_unit), low2 = __float2half2_rn(low * per_unit);
+          const float up = per_unit * kPValTop;
+          const __half2 s2 = __float2half2_rn(step * up), low2 = __float2half2_rn(low * up);
 #pragma unroll 1
           for (int u = 0; u < kWords; ++u) {
             const int to = part * kWords + u;

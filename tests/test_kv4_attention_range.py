@@ -171,3 +171,11 @@ def _large_row(dev, hd, rows, size, part):
 @pytest.mark.parametrize("hd", [32, 64, 128])
 def test_one_strong_key_before_a_long_cache_of_a_prompt(dev, hd, rows, drop):
     _strong_key(dev, hd, rows, drop, 200)
+
+
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("size", [30.0, 3e3, 6e4])
+@pytest.mark.parametrize("part", [0, 1])
+def test_a_large_row_moves_none_of_a_prompt_that_does_not_see_it(dev, hd, rows, size, part):
+    _large_row(dev, hd, rows, size, part)
