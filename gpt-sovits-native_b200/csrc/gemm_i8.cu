@@ -25,6 +25,8 @@ __device__ __forceinline__ void load8(const float* p, float* f) {
   for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(u[i]);
 }
 
+// One code by division.  Where the scale is a few units of fp32's last place the quotient may pass 127.
+__device__ __forceinline__ float code_of(float x, float s) { return fminf(fmaxf(__fdiv_rn(x, s), -127.f), 127.f); }
 // 8 codes of a row with scale s > 0.  x * (1 / s) is within 1e-4 of the quotient (below 128): further than that from a tie
 // it rounds like the quotient, else the division itself is made, as for a scale so small that its inverse is infinite.  A
 // sum with 1.5 2^23 is rounded to an integer, to even, with the code as its low byte.
@@ -39,7 +41,7 @@ __device__ __forceinline__ uint2 codes8(const float* x, float s, float per_s) {
   }
   if (!(far < 0.4998f) || per_s > 3.0e38f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = __fdiv_rn(x[i], s) + kRound;
+    for (int i = 0; i < 8; ++i) c[i] = code_of(x[i], s) + kRound;
   }
   uint32_t w[2];
 #pragma unroll
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(256)
     *reinterpret_cast<uint2*>(qr + 8 * i) = some ? codes8(f, s, per_s) : make_uint2(0, 0);
   }
   for (int i = 8 * whole + tid; i < n; i += THREADS)
-    qr[i] = some ? static_cast<int8_t>(rintf(__fdiv_rn(as_f32(xr[i]), s))) : 0;
+    qr[i] = some ? static_cast<int8_t>(rintf(code_of(as_f32(xr[i]), s))) : 0;
 }
 
 template <typename T>

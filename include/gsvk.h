@@ -789,7 +789,7 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* args, gsvk_stream_t stream
 /* ---- 8-bit integer products --------------------------------------------- */
 /* Row quantiser for gsvk_gemm_i8, for activations (per token) and weights
  * (per output channel): scale = max |x| / 127, q = rint(x / scale) (0 where
- * the scale is 0), fp32 arithmetic with IEEE division.  A row with a NaN or
+ * the scale is 0, no further than -127 and 127), fp32 arithmetic with IEEE division.  A row with a NaN or
  * an infinity gets q = 0 and scale = NaN.  x: fp32 when is_f32, else fp16 bits, rows
  * ldx elements apart (0: n); q rows ldq bytes apart (0: n), scale fp32 [rows].
  * Columns n .. ldq of a row are left as they are. */

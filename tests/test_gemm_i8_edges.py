@@ -20,3 +20,19 @@ def test_rows_whose_scale_has_no_finite_inverse(dev, rows, n, pad, top):
         q, scale = dev.quantize_rows_i8(torch.from_numpy(x).cuda()[:, :n])
         np.testing.assert_array_equal(scale.cpu().numpy(), s)
         np.testing.assert_array_equal(q.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,pad", [(1, 8, 0), (700, 512, 0), (5, 1024, 8), (64, 4096, 0), (2, 20001, 7), (9, 1001, 3)])
+def test_codes_stop_at_127(dev, rows, n, pad):
+    """Near the smallest subnormals a scale is a few units of its last place, and x / scale passes 127: 190 units over 127
+    are 1.496, a scale of 1."""
+    tiny = np.finfo(np.float32).smallest_subnormal
+    rng = np.random.default_rng(n)
+    x = rng.integers(-190, 191, (rows, n + pad)).astype(np.float32) * tiny
+    x[:, 2], x[:, n - 1] = 190 * tiny, -190 * tiny
+    s = np.abs(x[:, :n]).max(1) / np.float32(127)
+    assert (s == tiny).all()
+    q, scale = dev.quantize_rows_i8(torch.from_numpy(x).cuda()[:, :n])
+    np.testing.assert_array_equal(scale.cpu().numpy(), s)
+    np.testing.assert_array_equal(q.cpu().numpy(), np.clip(np.rint(x[:, :n] / tiny), -127, 127).astype(np.int8))
