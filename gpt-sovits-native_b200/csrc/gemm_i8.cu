@@ -136,8 +136,13 @@ struct I8Epilogue {
   float slope;
 };
 
+// GELU from q = gelu_tail(x): x Phi(x) = max(x, 0) - |x| q, with |x| no further than gelu_tail follows it.  So infinity
+// times 0 does not make NaN of the limits (infinity and 0), and past 5.5, where the result is below 1.1e-7, the bound takes
+// back part of what q is too large by.  NaN stays.
+__device__ __forceinline__ float gelu_from(float x, float q) { return fmaf(-fminf(fabsf(x), 5.5f), q, max_nan(x, 0.f)); }
 __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bias, const I8Epilogue& e) {
-  return apply_act(fmaf(static_cast<float>(acc), sa * sb, bias), e.act, e.slope);
+  const float y = fmaf(static_cast<float>(acc), sa * sb, bias);
+  return e.act == GSVK_ACT_GELU_ERF ? gelu_from(y, gelu_tail(y)) : apply_act(y, e.act, e.slope);
 }
 
 // ------------------------------------------------------------- tensor cores
@@ -192,7 +197,7 @@ __device__ __forceinline__ uint8_t* unit16(uint8_t* tile, int r, int j) {
   return tile + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
 }
 
-// GELU of 16 values, two to an operation: gelu_erf's Phi(-u) (common.cuh) as x Phi(x) = max(x, 0) - |x| Phi(-|x|).
+// GELU of 16 values, two to an operation: gelu_tail (common.cuh) and gelu_from, bit for bit.
 __device__ __forceinline__ void gelu16(float* v) {
 #pragma unroll
   for (int j = 0; j < 16; j += 2) {
@@ -212,8 +217,8 @@ __device__ __forceinline__ void gelu16(float* v) {
     float q0, q1;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(e.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(e.y));
-    v[j] = fmaf(-fabsf(v[j]), q0, max_nan(v[j], 0.f));
-    v[j + 1] = fmaf(-fabsf(v[j + 1]), q1, max_nan(v[j + 1], 0.f));
+    v[j] = gelu_from(v[j], q0);
+    v[j + 1] = gelu_from(v[j + 1], q1);
   }
 }
 

@@ -36,3 +36,46 @@ def test_codes_stop_at_127(dev, rows, n, pad):
     q, scale = dev.quantize_rows_i8(torch.from_numpy(x).cuda()[:, :n])
     np.testing.assert_array_equal(scale.cpu().numpy(), s)
     np.testing.assert_array_equal(q.cpu().numpy(), np.clip(np.rint(x[:, :n] / tiny), -127, 127).astype(np.int8))
+
+
+def _both_paths(dev, a, b, sa, sb, **kw):
+    """The product of rows in whole 16 bytes (tensor cores) and of the same rows an odd stride apart (CUDA cores)."""
+    out = []
+    for odd in (0, 1):
+        t = []
+        for x in (a, b):
+            wide = torch.zeros(x.shape[0], x.shape[1] + odd, dtype=torch.int8, device="cuda")
+            wide[:, :x.shape[1]] = x
+            t.append(wide[:, :x.shape[1]])
+        c = torch.empty(a.shape[0], b.shape[0], device="cuda")
+        h = torch.empty_like(c, dtype=torch.float16)
+        dev.gemm_i8(t[0], sa, t[1], sb, c=c, c_f16=h, **kw)
+        out.append((c, h))
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("M,N,K", [(70, 70, 64), (300, 520, 256), (1, 33, 16)])
+def test_both_paths_give_the_same_bits(dev, M, N, K, act):
+    gen = torch.Generator().manual_seed(act + M)
+    a, b = (torch.randint(-127, 128, (r, K), generator=gen, dtype=torch.int8).cuda() for r in (M, N))
+    sa, sb = (torch.rand(r, generator=gen).mul(0.03).cuda() for r in (M, N))
+    bias, res = torch.randn(N, generator=gen).cuda(), torch.randn(M, N, generator=gen).cuda()
+    bias[0], bias[-1], sa[M // 2] = float("inf"), float("-inf"), float("nan")
+    for kw in (dict(), dict(residual=res)):
+        (c0, h0), (c1, h1) = _both_paths(dev, a, b, sa, sb, bias=bias, act=act, slope=0.1, **kw)
+        for x, y in ((c0, c1), (h0, h1)):
+            np.testing.assert_array_equal(x.cpu().numpy(), y.cpu().numpy())
+
+
+@pytest.mark.gpu
+def test_gelu_at_the_infinities(dev):
+    """x Phi(x): inf at inf, 0 at -inf and far below 0, NaN for NaN; what is large and finite stays."""
+    one = torch.ones(4, device="cuda")
+    a, b = torch.zeros(4, 16, dtype=torch.int8, device="cuda"), torch.zeros(8, 16, dtype=torch.int8, device="cuda")
+    inf = float("inf")
+    bias = torch.tensor([inf, -inf, float("nan"), 3e38, -3e38, 1e20, -1e20, 0.0], device="cuda")
+    want = np.array([inf, 0, np.nan, 3e38, 0, 1e20, 0, 0], np.float32)
+    for c, _ in _both_paths(dev, a, b, one, torch.ones(8, device="cuda"), bias=bias, act=2):
+        np.testing.assert_array_equal(c.cpu().numpy(), np.tile(want, (4, 1)))
