@@ -164,7 +164,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // x Phi(x) (under one ulp of the result) and within 2.4e-6 relative where
 // |GELU(x)| > 1e-6.  The clamp leaves the exact -x^2 term, so past
 // |x| = 5.5 it only perturbs values smaller than 1.1e-7.
-__device__ __forceinline__ float gelu_tail(float x) {  // Phi(-|x|)
+__device__ __forceinline__ float gelu_erf(float x) {
   const float u = fminf(fabsf(x), 5.5f);
   float h = -1.725302567e-08f;
   h = fmaf(h, u, 5.477549507e-07f);
@@ -177,12 +177,8 @@ __device__ __forceinline__ float gelu_tail(float x) {  // Phi(-|x|)
   h = fmaf(h, u, 2.621913850e-01f);
   h = fmaf(h, u, -1.151113272e+00f);
   h = fmaf(h, u, -9.999998212e-01f);
-  float q;
+  float q;  // Phi(-|x|)
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(-0.721347520444f, x * x, h)));
-  return q;
-}
-__device__ __forceinline__ float gelu_erf(float x) {
-  const float q = gelu_tail(x);
   return x * (x >= 0.f ? 1.f - q : q);
 }
 // tanh stays out of line: epilogues unroll apply_act per element, and

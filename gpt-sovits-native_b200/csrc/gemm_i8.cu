@@ -136,13 +136,36 @@ struct I8Epilogue {
   float slope;
 };
 
-// GELU from q = gelu_tail(x): x Phi(x) = max(x, 0) - |x| q, with |x| no further than gelu_tail follows it.  So infinity
-// times 0 does not make NaN of the limits (infinity and 0), and past 5.5, where the result is below 1.1e-7, the bound takes
-// back part of what q is too large by.  NaN stays.
-__device__ __forceinline__ float gelu_from(float x, float q) { return fmaf(-fminf(fabsf(x), 5.5f), q, max_nan(x, 0.f)); }
+// GELU of two values, two to an operation: gelu_erf's q = Phi(-|x|) (common.cuh) as x Phi(x) = max(x, 0) - |x| q, with |x|
+// no further than q's polynomial follows it.  So infinity times 0 does not make NaN of the limits (infinity and 0), and past
+// 5.5, where the result is below 1.1e-7, the bound takes back part of what q is too large by.  NaN stays.
+__device__ __forceinline__ void gelu2(float& v0, float& v1) {
+  const uint64_t x = pair(v0, v1);
+  const float u0 = fminf(fabsf(v0), 5.5f), u1 = fminf(fabsf(v1), 5.5f);
+  const uint64_t u = pair(u0, u1);
+  uint64_t h = pair(-1.725302567e-08f, -1.725302567e-08f);
+  h = fma2(h, u, pair(5.477549507e-07f, 5.477549507e-07f));
+  h = fma2(h, u, pair(-7.458289474e-06f, -7.458289474e-06f));
+  h = fma2(h, u, pair(5.484473149e-05f, 5.484473149e-05f));
+  h = fma2(h, u, pair(-2.005067072e-04f, -2.005067072e-04f));
+  h = fma2(h, u, pair(-1.761470485e-04f, -1.761470485e-04f));
+  h = fma2(h, u, pair(7.180649787e-03f, 7.180649787e-03f));
+  h = fma2(h, u, pair(-5.261564627e-02f, -5.261564627e-02f));
+  h = fma2(h, u, pair(2.621913850e-01f, 2.621913850e-01f));
+  h = fma2(h, u, pair(-1.151113272e+00f, -1.151113272e+00f));
+  h = fma2(h, u, pair(-9.999998212e-01f, -9.999998212e-01f));
+  const float2 e = unpair(fma2(mul2(x, x), pair(-0.721347520444f, -0.721347520444f), h));
+  float q0, q1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(e.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(e.y));
+  v0 = fmaf(-u0, q0, max_nan(v0, 0.f));
+  v1 = fmaf(-u1, q1, max_nan(v1, 0.f));
+}
 __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bias, const I8Epilogue& e) {
-  const float y = fmaf(static_cast<float>(acc), sa * sb, bias);
-  return e.act == GSVK_ACT_GELU_ERF ? gelu_from(y, gelu_tail(y)) : apply_act(y, e.act, e.slope);
+  float y = fmaf(static_cast<float>(acc), sa * sb, bias), same = y;
+  if (e.act != GSVK_ACT_GELU_ERF) return apply_act(y, e.act, e.slope);
+  gelu2(y, same);
+  return y;
 }
 
 // ------------------------------------------------------------- tensor cores
@@ -197,29 +220,9 @@ __device__ __forceinline__ uint8_t* unit16(uint8_t* tile, int r, int j) {
   return tile + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
 }
 
-// GELU of 16 values, two to an operation: gelu_tail (common.cuh) and gelu_from, bit for bit.
 __device__ __forceinline__ void gelu16(float* v) {
 #pragma unroll
-  for (int j = 0; j < 16; j += 2) {
-    const uint64_t x = pair(v[j], v[j + 1]), u = pair(fminf(fabsf(v[j]), 5.5f), fminf(fabsf(v[j + 1]), 5.5f));
-    uint64_t h = pair(-1.725302567e-08f, -1.725302567e-08f);
-    h = fma2(h, u, pair(5.477549507e-07f, 5.477549507e-07f));
-    h = fma2(h, u, pair(-7.458289474e-06f, -7.458289474e-06f));
-    h = fma2(h, u, pair(5.484473149e-05f, 5.484473149e-05f));
-    h = fma2(h, u, pair(-2.005067072e-04f, -2.005067072e-04f));
-    h = fma2(h, u, pair(-1.761470485e-04f, -1.761470485e-04f));
-    h = fma2(h, u, pair(7.180649787e-03f, 7.180649787e-03f));
-    h = fma2(h, u, pair(-5.261564627e-02f, -5.261564627e-02f));
-    h = fma2(h, u, pair(2.621913850e-01f, 2.621913850e-01f));
-    h = fma2(h, u, pair(-1.151113272e+00f, -1.151113272e+00f));
-    h = fma2(h, u, pair(-9.999998212e-01f, -9.999998212e-01f));
-    const float2 e = unpair(fma2(mul2(x, x), pair(-0.721347520444f, -0.721347520444f), h));
-    float q0, q1;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q0) : "f"(e.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q1) : "f"(e.y));
-    v[j] = gelu_from(v[j], q0);
-    v[j + 1] = gelu_from(v[j + 1], q1);
-  }
+  for (int j = 0; j < 16; j += 2) gelu2(v[j], v[j + 1]);
 }
 
 template <int BN>
