@@ -161,8 +161,11 @@ __device__ __forceinline__ void gelu2(float& v0, float& v1) {
   v0 = fmaf(-u0, q0, max_nan(v0, 0.f));
   v1 = fmaf(-u1, q1, max_nan(v1, 0.f));
 }
+// ReLU that keeps the NaN of a bad row's scale, which v > 0 ? v : 0 would make an ordinary 0.
+__device__ __forceinline__ float relu_nan(float v) { return max_nan(v, 0.f); }
 __device__ __forceinline__ float i8_value(int acc, float sa, float sb, float bias, const I8Epilogue& e) {
   float y = fmaf(static_cast<float>(acc), sa * sb, bias), same = y;
+  if (e.act == GSVK_ACT_RELU) return relu_nan(y);
   if (e.act != GSVK_ACT_GELU_ERF) return apply_act(y, e.act, e.slope);
   gelu2(y, same);
   return y;
@@ -386,6 +389,9 @@ __global__ void __launch_bounds__(kI8Threads<BN>, 1)
           }
           if (e.act == GSVK_ACT_GELU_ERF) {
             gelu16(v);
+          } else if (e.act == GSVK_ACT_RELU) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = relu_nan(v[j]);
           } else {
             act_array<16>(v, e.act, e.slope);
           }

@@ -79,3 +79,18 @@ def test_gelu_at_the_infinities(dev):
     want = np.array([inf, 0, np.nan, 3e38, 0, 1e20, 0, 0], np.float32)
     for c, _ in _both_paths(dev, a, b, one, torch.ones(8, device="cuda"), bias=bias, act=2):
         np.testing.assert_array_equal(c.cpu().numpy(), np.tile(want, (4, 1)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
+def test_a_bad_row_shows_through_every_activation(dev, act):
+    """The scale of a row with a NaN or an infinity is NaN: no activation may make an ordinary row of it."""
+    x = torch.randn(40, 96, generator=torch.Generator().manual_seed(3)).half().cuda()
+    x[7, 3], x[9, 0] = float("nan"), float("inf")
+    w, ws = dev.quantize_rows_i8(torch.randn(50, 96, generator=torch.Generator().manual_seed(4)).cuda())
+    q, s = dev.quantize_rows_i8(x)
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[7, 9]] = True
+    for c, h in _both_paths(dev, q, w, s, ws, act=act, slope=0.1):
+        for y in (c, h):
+            assert y[bad].isnan().all() and y[~bad].isfinite().all()
