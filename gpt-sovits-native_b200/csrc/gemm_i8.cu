@@ -553,7 +553,8 @@ int gsvk_gemm_i8(const gsvk_gemm_i8_args* g, gsvk_stream_t stream) {
   if (!g || !g->a || !g->b || !g->a_scale || !g->b_scale || (!g->c && !g->c_f16))
     return fail(GSVK_ERR_INVALID, "gemm_i8: null pointer");
   if (g->N == 0 || g->K == 0) return fail(GSVK_ERR_INVALID, "gemm_i8: zero size");
-  if (g->M > 0x7fffff00 || g->N > 0x7fffff00 || g->K >= 131072)
+  // a grid of the CUDA-core kernel, and 128 x 32 tiles of the other, count up to 2^31 - 1; M N is below 2^62
+  if (g->M > 0x7fffff00 || g->N > 0x7fffff00 || g->K >= 131072 || (g->M * g->N + 255) / 256 > 0x7fffffff)
     return fail(GSVK_ERR_UNSUPPORTED, "gemm_i8: %zu x %zu x %zu (K below 131072: 32-bit sums)", g->M, g->N, g->K);
   const size_t lda = g->lda ? g->lda : g->K, ldb = g->ldb ? g->ldb : g->K;
   const size_t ldc = g->ldc ? g->ldc : g->N, ldh = g->ldc_f16 ? g->ldc_f16 : g->N;
@@ -577,7 +578,6 @@ int gsvk_gemm_i8(const gsvk_gemm_i8_args* g, gsvk_stream_t stream) {
     return launch_i8<32>(g, sa, sb, e, st);
   }
   const size_t outs = g->M * g->N;
-  if (ceil_div(outs, 256) > 0x7fffffff) return fail(GSVK_ERR_UNSUPPORTED, "gemm_i8: too big");
   gemm_i8_simt_kernel<<<ceil_div(outs, 256), 256, 0, st>>>(
       g->a, (long long)lda, g->b, (long long)ldb, (long long)g->M, (int)g->N, (int)g->K, e);
   return check_launch("gemm_i8_simt_kernel");

@@ -94,3 +94,15 @@ def test_a_bad_row_shows_through_every_activation(dev, act):
     for c, h in _both_paths(dev, q, w, s, ws, act=act, slope=0.1):
         for y in (c, h):
             assert y[bad].isnan().all() and y[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("M,N", [(2**31 - 300, 2**31 - 300), (2**30, 2**30), (2**25, 2**24), (2**20 + 1, 2**19)])
+def test_more_outputs_than_a_launch_holds_are_refused(gsv, M, N):
+    """A block count past 32 bits must not wrap to a small grid."""
+    import ctypes
+
+    from gsv_b200.quant import GemmI8Args
+
+    for ld in (64, 65):
+        g = GemmI8Args(a=256, lda=ld, b=256, ldb=ld, a_scale=256, b_scale=256, M=M, N=N, K=64, c=256, ldc=N)
+        assert gsv.lib().gsvk_gemm_i8(ctypes.byref(g), None) == -5
