@@ -266,13 +266,13 @@ __global__ void __launch_bounds__(kPlanThreads)
   for (int i = warp; i < n_seq; i += kPlanThreads / 32) {
     const int n = blocks_of(i);
     int32_t* row = table + static_cast<size_t>(i) * max_blocks;
-    int to = rel_smem[i];
+    unsigned to = static_cast<unsigned>(rel_smem[i]);  // up to n_pages and a row more: past 2^31 - 1
     for (int b = 0; b < n; b += 32) {
       const int page = b + lane < n ? row[b + lane] : -1;
       const bool ok = page >= 0 && page < n_pages;
       const unsigned m = __ballot_sync(0xffffffffu, ok);
-      const int place = to + __popc(m & ((1u << lane) - 1u));
-      if (ok && place < n_pages) free_pages[place] = page;
+      const unsigned place = to + __popc(m & ((1u << lane) - 1u));
+      if (ok && place < static_cast<unsigned>(n_pages)) free_pages[place] = page;
       if (b + lane < n) row[b + lane] = -1;
       to += __popc(m);
     }
