@@ -67,6 +67,7 @@ template <int HD>
 constexpr int kTileBytes = kTile * (HD + 8);
 template <int HD>
 constexpr int kRecord = HD + 4;  // floats of a joined row: maximum, sum, (pad), values
+constexpr int kRecords = 3;      // of a warp
 // Scores (two keys each, 64 bits) or weights (two fp16 each, first and second part) of a row between
 // the products: 32 pairs, and 32 bytes that keep eight rows off each other's banks.
 constexpr int kRowBytes = 32 * 8 + 32;
@@ -338,6 +339,31 @@ __device__ __forceinline__ void add_tile(const uint8_t* tile, uint8_t* mid, int 
   }
 }
 
+// A warp's records, ROWS rows each: of its first item, if that began in another warp; of its last one, if that goes on in
+// the next, or of one of more than kSumKeys keys; and of the latest of such an item's keys.
+template <int HD, int ROWS>
+__device__ __forceinline__ float* record_of(const AttnArgs& a, int warp, int i) {
+  return a.parts + (static_cast<size_t>(warp) * kRecords + i) * ROWS * kRecord<HD>;
+}
+// Adds a record's rows to another's: a lane to head_dim / 32 dimensions.
+template <int HD>
+__device__ __forceinline__ void add_record(float* to, const float* from, int rows, int lane) {
+#pragma unroll 1
+  for (int row = 0; row < rows; ++row, to += kRecord<HD>, from += kRecord<HD>) {
+    const float2 x = *reinterpret_cast<const float2*>(to), y = *reinterpret_cast<const float2*>(from);
+    __syncwarp();
+    const float top = fmaxf(x.x, y.x), base = top == -INFINITY ? 0.f : top;
+    const float by = ex2(x.x - base), by1 = ex2(y.x - base);
+    if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(top, fmaf(x.y, by, y.y * by1));
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d) {
+      float* v = to + 4 + lane + 32 * d;
+      *v = fmaf(*v, by, from[4 + lane + 32 * d] * by1);
+    }
+  }
+  __syncwarp();
+}
+
 // Joins the pieces of an item (records of warps first .. last) in their order: a lane to head_dim / 32 dimensions.  The
 // loads of up to four rows and four pieces are in flight together; row by row and two pieces at a time the join was most
 // of a short call's time (64 requests of 1,000 to 2,000 keys, 16 rows on 8 heads of 32: 58 us, 76 so).
@@ -346,13 +372,13 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, const Request& rq
                                             int lane) {
   constexpr int kD = HD / 32, kSide = ROWS < 4 ? ROWS : 4, kAhead = kSide > 1 && HD == 128 ? 2 : 4;
   const int rows = min(ROWS, rq.n * a.group - block * ROWS), n = last - first + 1;
-  const size_t stride = static_cast<size_t>(2) * ROWS * kRecord<HD>;  // from a warp's records to the next's
+  const size_t stride = static_cast<size_t>(kRecords) * ROWS * kRecord<HD>;  // from a warp's records to the next's
 #pragma unroll 1
   for (int row0 = 0; row0 < rows; row0 += kSide) {
     // the first warp's piece is its last one (second record), the others' their first; rows past the last hold
     // numbers of no meaning and are not written
-    const float* r0 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + ROWS + row0) * kRecord<HD>;
-    const float* r1 = a.parts + (static_cast<size_t>(first) * 2 * ROWS + row0) * kRecord<HD>;
+    const float* r0 = record_of<HD, ROWS>(a, first, 1) + row0 * kRecord<HD>;
+    const float* r1 = record_of<HD, ROWS>(a, first, 0) + row0 * kRecord<HD>;
     float base[kSide], sum[kSide], acc[kSide][kD];
 #pragma unroll
     for (int k = 0; k < kSide; ++k) base[k] = -INFINITY;
@@ -471,7 +497,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
   bool alive = true;
 #pragma unroll 1
   while (u < run) {
-    const int t1 = min(at.tiles, at.tile + (run - u));
+    const int t1 = min(min(at.tiles, at.tile + (run - u)), at.tile + kSumKeys / kTile);
     load_rows<HD, ROWS>(a, at.req, at.head, at.block, lane, s);
     const int all = at.req.n * a.group, rows = min(ROWS, all - at.block * ROWS);
     const int limit = limit_of(a, at.req, min(at.block * ROWS + lane, all - 1));  // of row `lane`
@@ -494,6 +520,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
     if (!alive) break;
     // the item's rows so far: sums over the lanes of a row, and the codes' unit
     const bool whole = at.tile == 0 && t1 == at.tiles;
+    // keys of this run that are in the item's record already: these go into the third one, and from there to them
+    const bool earlier = at.tile > max(0, -item_start);
     // the warps that share the item
     const int first = me - (item_start < 0 ? (share - 1 - item_start) / share : 0);
     const int last = me + (item_start + at.tiles - 1) / share;
@@ -530,7 +558,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
             *reinterpret_cast<uint4*>(o + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
           }
         } else {
-          float* r = a.parts + (static_cast<size_t>(me) * 2 * ROWS + (me == first ? ROWS : 0) + in_block) * kRecord<HD>;
+          float* r = record_of<HD, ROWS>(a, me, earlier ? 2 : me == first ? 1 : 0) + in_block * kRecord<HD>;
           if ((lane & 3) == 0) *reinterpret_cast<float2*>(r) = make_float2(m, l);
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i)
@@ -540,15 +568,24 @@ __global__ void __launch_bounds__(kSplitWarps * 32, kCtasPerSm<HD, ROWS>) kv4_at
       }
     }
     if (!whole) {
+      if (earlier) {
+        __syncwarp();
+        add_record<HD>(record_of<HD, ROWS>(a, me, me == first ? 1 : 0), record_of<HD, ROWS>(a, me, 2), rows, lane);
+      }
+      if (t1 < at.tiles && u < run) {  // more of the item in this run
+        at.tile = t1;
+        continue;
+      }
       __threadfence();
       __syncwarp();
       int n = 0;
-      if (lane == 0) n = atomicAdd(a.tickets + first, 1);
+      // an item of this warp alone takes no ticket: that place is the last item's, which others may have drawn from
+      if (lane == 0 && first != last) n = atomicAdd(a.tickets + first, 1);
       n = __shfl_sync(0xffffffffu, n, 0);
       if (n == last - first) {
         __threadfence();
         join_pieces<HD, ROWS>(a, at.req, at.head, at.block, first, last, lane);
-        if (lane == 0) a.tickets[first] = 0;
+        if (lane == 0 && first != last) a.tickets[first] = 0;
       }
     }
     item_start += at.tiles;
@@ -609,7 +646,7 @@ size_t gsvk_kv4_attention_workspace(size_t n_seq, size_t n_tokens, size_t heads,
       heads == 0 || heads > 65536 || n_tokens > 0x7fffffff / (heads / kv_heads) ||
       (head_dim != 32 && head_dim != 64 && head_dim != 128))
     return 0;
-  return attention_parts() + split_warps(head_dim) * 2 * 16 * (head_dim + 4) * sizeof(float) +
+  return attention_parts() + split_warps(head_dim) * kRecords * 16 * (head_dim + 4) * sizeof(float) +
          (may_be_long(n_tokens, heads / kv_heads) ? kv4_prompt_part_bytes(head_dim) : 0);
 }
 
@@ -662,7 +699,7 @@ int gsvk_kv4_attention(const gsvk_kv4_attention_args* g, gsvk_stream_t stream) {
   uint8_t* ws = static_cast<uint8_t*>(g->workspace);
   a.long_tickets = reinterpret_cast<int*>(ws + tickets_bytes());
   a.parts = reinterpret_cast<float*>(ws + attention_parts());
-  a.long_parts = reinterpret_cast<float*>(ws + attention_parts() + split_warps(hd) * 2 * 16 * (hd + 4) * sizeof(float));
+  a.long_parts = reinterpret_cast<float*>(ws + attention_parts() + split_warps(hd) * kRecords * 16 * (hd + 4) * sizeof(float));
   a.status = device_status();
   cudaStream_t st = as_cuda(stream);
   // Requests with more rows than this take the kernel with 128-row tiles.

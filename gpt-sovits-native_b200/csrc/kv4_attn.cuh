@@ -28,6 +28,11 @@ struct AttnArgs {
   int most_rows;     // rows of a request (to a kv head) that the few-row kernel takes
 };
 
+// Keys of one sum on the tensor cores.  They cut each step of 16 keys off at 24 bits, so that a sum whose terms do not
+// cancel shrinks by up to 2^-24 a step: 2^-14 over these keys in two parts, 3.5e-4 over 60,000.  What a worker has of an
+// item past these keys is put into its record, rounded, and summed anew.
+constexpr int kSumKeys = 8192;
+
 // One request's rows and the keys they see.
 struct Request {
   int q0, n, len, prefix;

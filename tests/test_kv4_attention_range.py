@@ -179,3 +179,34 @@ def test_one_strong_key_before_a_long_cache_of_a_prompt(dev, hd, rows, drop):
 @pytest.mark.parametrize("part", [0, 1])
 def test_a_large_row_moves_none_of_a_prompt_that_does_not_see_it(dev, hd, rows, size, part):
     _large_row(dev, hd, rows, size, part)
+
+
+def _long_sums(dev, hd, rows, copies):
+    """60,000 keys whose values are positive; or whose greatest code stands for 0, in a channel that has no other: what a
+    kernel sums does not cancel, the result does, and shows it.  An item's sums are long where it is one run.  The bound:
+    the result's rounding, the weights' to 11 bits (each by chance, so 2^-11 / sqrt(10,000 keys that count) of the
+    values), and 2^-14 for sums of 8,192 keys in steps of 16 that are cut off at 24 bits, 2^-24 each at most on average, in
+    one part or two (1,024 2^-24)."""
+    gen = torch.Generator().manual_seed(6)
+    length = 60000
+    c = Cache(length, hd)
+    _octaves(c, torch.rand(length, generator=gen) * 2 - 1)
+    c.code[1] = torch.randint(0, 16, (length, hd), generator=gen, dtype=torch.uint8)
+    c.code[1, :, 0], c.code[1, :, 1] = 15, 0
+    c.code[1, :, 2] = torch.randint(12, 16, (length,), generator=gen)
+    c.step[1] = (torch.rand(length, generator=gen) * 0.02 + 0.05).half()
+    q = torch.ones(rows, 1, hd, dtype=torch.float16, device="cuda")
+    for low in (1.1, -15.0):
+        c.low[1] = (torch.full((length,), low) if low > 0 else low * c.step[1].float()).half()
+        got = _attend(dev, c, q, LN2, copies=copies)
+        want, _ = _exact(c, q, LN2, 22)
+        size = (c.values()[1].abs().mean(0) + 8 * 0.06)  # of a channel's terms, in values or centred codes
+        bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 * 0.01 + 2.0 ** -14) * size
+        off = (got - want).abs() / bound
+        assert (off <= 1).all(), (low, float(off.max()))
+
+
+@pytest.mark.parametrize("rows,copies", [(1, 1), (1, 64), (1, 3000), (4, 1200), (7, 1600), (16, 1600)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_sums_of_one_sign(dev, hd, rows, copies):
+    _long_sums(dev, hd, rows, copies)
