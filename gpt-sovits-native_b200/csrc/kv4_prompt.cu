@@ -60,6 +60,8 @@ constexpr int kPTile = HD <= 64 ? 128 : 64;  // keys
 template <int HD>
 constexpr int kPTileShift = HD <= 64 ? 7 : 6;
 template <int HD>
+constexpr int kPSumTiles = kSumKeys / kPTile<HD>;  // of one item's sums; with more it counts as several items of the same rows
+template <int HD>
 constexpr bool kPSide = HD == 32;  // their parts side by side, in sums of their own; else both into the same sums
 template <int HD>
 constexpr int kPCols = kPSplit<HD> ? 2 * HD : HD;  // columns of the value operand
@@ -367,7 +369,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       const bool live_row = row < all, active = block < blocks;
       const int limit = limit_of(a, at.req, min(row, all - 1));
       const int least = __reduce_min_sync(0xffffffffu, limit);
-      const int t0 = at.tile, t1 = min(at.tiles, t0 + run - g);
+      const int t0 = at.tile, t1 = min(min(at.tiles, t0 + run - g), t0 + kPSumTiles<HD>);
       float ref = -INFINITY, unit = 0.f, tile_sum = 0.f;
       uint64_t l2 = 0, pb2 = 0;
       for (int i = t0; i < t1; ++i, ++g) {
@@ -537,9 +539,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         ++mine;
       }
       if (!ok) break;
-      // the next item's queries, over those that the last scores have used, while the last sums are made
+      // the next item's queries, over those that the last scores have used, while the last sums are made; or more of this
+      // item's keys
       const typename L::Cursor done = at;
-      if (g < run) {
+      const bool more = t1 < done.tiles && g < run;
+      if (more) {
+        at.tile = t1;
+        if (active && lane == 0) mbar_arrive(&q_full[block]);
+      } else if (g < run) {
         at.next_item(a);
         if (block < blocks_of(at)) {
           uint4 x[HD / 8];
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         }
       }
       const int start = item_start;
-      item_start += done.tiles;
+      if (!more) item_start += done.tiles;
       if (!active) continue;
       ok = mbar_wait(&o_full[block], static_cast<uint32_t>(items) & 1u, a.status);
       ok = __all_sync(0xffffffffu, ok);
@@ -565,6 +572,17 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       uint16_t* out = out_row(a, done.req, done.head, live_row ? row : all - 1, HD);
       // a CTA's records: its last item's, if that goes on in the next CTA, then its first's
       float4* record = reinterpret_cast<float4*>(a.long_parts + (static_cast<size_t>(me) * 2 + (me == first ? 0 : 1)) * kPRows * kPRecord<HD>) + tid;
+      // in which it has the item's earlier keys already, where there are more than kSumKeys
+      const bool earlier = t0 > max(0, -start);
+      float by = 1.f, by0 = 0.f, all_l = l;
+      if (earlier) {
+        const float2 before = *reinterpret_cast<const float2*>(record);
+        const float top = fmaxf(ref, before.x), base = top == -INFINITY ? 0.f : top;
+        by = ex2(ref - base);
+        by0 = ex2(before.x - base);
+        ref = top;
+        all_l = fmaf(l, by, before.y * by0);
+      }
 #pragma unroll 1
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
@@ -586,8 +604,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
           if (whole) {
             if (live_row) put8(out + c + 8 * u, v);
           } else {
-            record[(1 + c / 4 + 2 * u) * kPRows] = make_float4(v[0], v[1], v[2], v[3]);
-            record[(2 + c / 4 + 2 * u) * kPRows] = make_float4(v[4], v[5], v[6], v[7]);
+            float4* r0 = record + (1 + c / 4 + 2 * u) * kPRows;
+            float4* r1 = r0 + kPRows;
+            if (earlier) {
+              const float4 x = *r0, y = *r1;
+              v[0] = fmaf(v[0], by, x.x * by0);
+              v[1] = fmaf(v[1], by, x.y * by0);
+              v[2] = fmaf(v[2], by, x.z * by0);
+              v[3] = fmaf(v[3], by, x.w * by0);
+              v[4] = fmaf(v[4], by, y.x * by0);
+              v[5] = fmaf(v[5], by, y.y * by0);
+              v[6] = fmaf(v[6], by, y.z * by0);
+              v[7] = fmaf(v[7], by, y.w * by0);
+            }
+            *r0 = make_float4(v[0], v[1], v[2], v[3]);
+            *r1 = make_float4(v[4], v[5], v[6], v[7]);
           }
         }
       }
@@ -595,16 +626,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[block]);
       if (!whole) {
-        *record = make_float4(ref, l, 0.f, 0.f);
+        *record = make_float4(ref, all_l, 0.f, 0.f);
+        if (more) continue;
         __threadfence();
         __syncwarp();
-        int* ticket = a.long_tickets + first * 8 + warp;  // of these 32 rows
+        // of these 32 rows; none of an item of this CTA alone, whose place is the last item's
+        int* ticket = a.long_tickets + first * 8 + warp;
         int n = 0;
-        if (lane == 0) n = atomicAdd(ticket, 1);
+        if (lane == 0 && first != last) n = atomicAdd(ticket, 1);
         n = __shfl_sync(0xffffffffu, n, 0);
         if (n == last - first) {  // the others' pieces are there: join them in the order of their keys
           __threadfence();
-          if (lane == 0) *ticket = 0;
+          if (lane == 0 && first != last) *ticket = 0;
           constexpr int kSet = kPRows * kPRecord<HD> / 4;  // vectors of a CTA's record
           const float4* p0 = reinterpret_cast<const float4*>(a.long_parts) + static_cast<size_t>(first) * 2 * kSet + tid;
           const float4* p1 = p0 + kSet;  // the other CTAs': their second records
@@ -866,7 +899,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
       g = 0;
       const int n_run = same(run);
       while (g < n_run && ok) {
-        const int blocks = same(blocks_of(at)), end = same(g + min(at.tiles, at.tile + n_run - g) - at.tile);
+        const int blocks = same(blocks_of(at));
+        const int end = same(g + min(min(at.tiles - at.tile, n_run - g), kPSumTiles<HD>));
         // Steps: the first block's tile, the second's, the next tile ...  The scores run ahead of the sums by the
         // ring, one block's by two tiles (there are two buffers of K): a softmax group finds its next scores done.
         const int lead = blocks == 2 ? kR : 2;
@@ -908,8 +942,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const AttnArgs
         }
         ++item;
         if (blocks == 2) ++item1;
+        at.tile += end - g;
         g = end;
-        if (ok && g < n_run) at.next_item(a);
+        if (ok && g < n_run && at.tile == at.tiles) at.next_item(a);
       }
     }
   }

@@ -210,3 +210,9 @@ def _long_sums(dev, hd, rows, copies):
 @pytest.mark.parametrize("hd", [32, 64, 128])
 def test_long_sums_of_one_sign(dev, hd, rows, copies):
     _long_sums(dev, hd, rows, copies)
+
+
+@pytest.mark.parametrize("rows,copies", [(40, 1), (40, 20), (40, 200), (200, 30), (300, 150)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_long_sums_of_one_sign_of_a_prompt(dev, hd, rows, copies):
+    _long_sums(dev, hd, rows, copies)
