@@ -14,7 +14,8 @@ attention, output projection, LayerNorm, ReLU feed-forward, LayerNorm) and the
 mask is its prefill's (t2s_engine.cpp:881-1034): the text prefix is seen by
 every row, the rest causally.  The batched engine (T2SBatch) keeps a dense
 fp16 cache per request and fp16 weights; this one trades their exactness
-(cache rows in 4 bits, operands in 8) for 0.31 of the cache and half of the
+(cache rows in 4 bits, operands in 8) and some speed (1.62 ms a step of 64
+requests of 529 tokens against 1.42) for 0.31 of the cache and half of the
 weights.
 
 A step makes no host read and leaves its lengths, tables and free pages on the
@@ -101,7 +102,8 @@ class T2SPaged:
         the number of rows), none of them more than max_q.  `prefix`: leading
         tokens seen by every row of the request.  Returns the rows after the
         last layer; requests refused for want of pages are counted in
-        self.plan.refused, keep their lengths and get rows of no meaning."""
+        self.plan.refused, keep their lengths, have -1 in self.plan.slots at
+        their rows and get rows of no meaning."""
         import torch
 
         # all that a layer would refuse: the plan below moves the lengths on, so nothing may fail after it

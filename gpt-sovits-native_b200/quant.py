@@ -260,7 +260,9 @@ def kv4_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
 
 class KV4Workspace:
     """Scratch of KV4Cache.attention for up to `n_seq` requests and `n_tokens`
-    rows; the layers of a model share one."""
+    rows; the layers of a model share one, as may models of any head_dim whose
+    calls do not overlap.  After a device-side wait that ran out
+    (device_status) its buffer has to be zeroed."""
 
     def __init__(self, n_seq: int, n_tokens: int, heads: int, kv_heads: int, head_dim: int,
                  device=None):
@@ -350,7 +352,7 @@ class KV4Cache:
         cache (gsvk_kv4_attention): request i owns rows q_start[i] to
         q_start[i + 1], sees kv_len[i] keys causally from the end and its
         first prefix[i] from every row.  `workspace`: a KV4Workspace of at
-        least these sizes.  Returns fp16 rows like q."""
+        least these sizes and of no smaller head_dim.  Returns fp16 rows like q."""
         import torch
 
         f16, i32, here = torch.float16, torch.int32, _home(self._index, "the cache")

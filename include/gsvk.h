@@ -693,10 +693,11 @@ size_t gsvk_kv4_page_bytes(int page_size, int kv_heads, int head_dim);
  * free_pages[0 .. *free_count) in the requests' order.  A request that is not
  * granted, whose length is negative, passes max_blocks pages or whose tokens end past
  * max_tokens is refused: it keeps its pages and its length (the latter kinds need no
- * pages in the sum above).  Results:
+ * pages in the sum above; a negative ctx_len counts as 0 and comes back as 0).  The slots of
+ * its rows are -1.  Results:
  *   q_start[n_seq + 1]   first row of each request in the step's packed rows
  *                        (refused ones included; a negative new_len counts as 0)
- *   kv_len[n_seq]        tokens cached after the step: ctx + new, or ctx where refused
+ *   kv_len[n_seq]        tokens cached after the step: ctx + new, or ctx (0 at least) where refused
  *   block_table          [n_seq][max_blocks], entries of the granted pages written
  *   slots[max_tokens]    slot of each packed row; -1 for refused rows and past the last
  *   free_left[1], refused[1]   pages left, requests refused
@@ -753,17 +754,25 @@ int gsvk_kv4_read(const gsvk_kv4_cache* cache, const int64_t* slots, size_t n_to
  * first prefix_i keys seen by every row, as in the T2S prefill
  * (t2s_engine.cpp:881-1034).  out = softmax(scale q.k) . v over those keys,
  * zeros where there is none.  Scores, statistics and sums are fp32, the
- * result is rounded to fp16 once; the weights go into the last product as fp16
- * (22 bits for requests of up to 16 rows to a kv head), against values less
- * their row's middle at head_dim 128, which moves the result by 2^-11 of the
- * values at most.  Keys past the limit are not read into the
- * result, whatever their page holds; entries of block_table outside
- * [0, n_pages) count as keys past the limit.  Rows outside every
+ * result is rounded to fp16 once.  Into the last product the weights go
+ *   for requests of up to 16 rows to a kv head with 22 bits, down to 2^-17 of the greatest (all
+ *   of them to within 2^-40 of it),
+ *   for longer ones as fp16, 2^-31 of the greatest being the least that counts: at head_dim 32
+ *   and 64 against the values, at 128 against values less their row's middle, which moves the
+ *   result by 2^-11 of the values at most.
+ * Sums on the tensor cores are cut off, not rounded, and end after 8,192 keys: 2^-14 of a sum at most.
+ * Keys past the limit are not read into the result, whatever their page holds; entries of block_table
+ * outside [0, n_pages) count as keys past the limit.  (Requests of more than 16 rows take 128 keys, 64 at
+ * head_dim 128, in units of the greatest that any row sees: a row may be off by 2^-24 of one that
+ * it does not see itself.)  Rows outside every
  * request are left as they are.  max_q: a bound on the longest request's rows, for
  * the choice of kernel (results hold for any value).
  * workspace: DEVICE, 256-byte aligned, gsvk_kv4_attention_workspace() bytes, zero before the
- * first call and left fit for the next (its tickets zero); calls that may overlap need one each.
- * Its size depends on the GPU and head_dim, not on the lengths: 22 to 60 MB. */
+ * first call and left fit for the next (its tickets zero), of whatever sizes and head_dim; after a
+ * wait that ran out (gsvk_device_status) it has to be zeroed again.  Calls that may overlap need one each.
+ * Its size depends on the GPU, on head_dim and on whether a request may have more than 16 rows to a
+ * kv head (n_tokens heads / kv_heads above 16): on 148 SMs 16, 23 or 30 MB for head_dim 32, 64
+ * or 128 if not, 27, 44 or 70 MB if so. */
 typedef struct {
   gsvk_kv4_cache cache;
   const uint16_t* q; size_t q_stride;     /* elements between rows, a multiple of 8 */
@@ -797,10 +806,11 @@ int gsvk_quantize_rows_i8(const void* x, int is_f32, size_t rows, size_t n, size
                           size_t ldq, float* scale, gsvk_stream_t stream);
 /* C[m, n] = act(a_scale[m] b_scale[n] sum_k A[m, k] B[n, k] + bias[n]) + residual[m, n]:
  * int8 operands, exact 32-bit sums (K below 131072), fp32 epilogue, written as fp32
- * and/or fp16.  Leading dimensions of 0 mean dense rows.  Operands that are
+ * and/or fp16 (up to 2^39 outputs).  Leading dimensions of 0 mean dense rows.  Operands that are
  * 16-byte aligned with leading dimensions in whole 16 bytes run on the
  * tensor cores (any K: what lies between K and the leading dimension is not
- * read), others on a CUDA-core kernel with the same results. */
+ * read), others on a CUDA-core kernel with the same bits.  The NaN of a bad row's
+ * scale shows through every act; GELU is infinity at infinity and 0 at minus infinity. */
 typedef struct {
   const int8_t* a; size_t lda;       /* [M, K] */
   const int8_t* b; size_t ldb;       /* [N, K] */
