@@ -185,6 +185,16 @@ def _allocator(stream):
     return empty
 
 
+def _filled():
+    """Waits for the fills of an object's own buffers, which calls on any stream
+    may then use: the caller has no other handle on them.  (A capture orders
+    its own.)"""
+    import torch
+
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream().synchronize()
+
+
 # ------------------------------------------------------------------ page plan
 class KVPlan:
     """Pages and slots of each step of up to `n_seq` requests, built on the GPU
@@ -211,6 +221,7 @@ class KVPlan:
             max_tokens=self.max_tokens, page_size=self.page_size, q_start=self.q_start.data_ptr(),
             slots=self.slots.data_ptr(), refused=self.refused.data_ptr(),
             workspace=self._ticket.data_ptr())
+        _filled()
 
     def _state(self, length, block_table, free_pages, free_count):
         import torch
@@ -276,6 +287,7 @@ class KV4Workspace:
                              f"over {kv_heads} of {head_dim}")
         self.buffer = torch.zeros(self.bytes, dtype=torch.uint8, device=device)
         self.ptr = self.buffer.data_ptr()
+        _filled()
 
 
 class KV4Cache:

@@ -140,3 +140,38 @@ def test_calls_run_where_the_current_device_is(dev, monkeypatch):
         for i in at:
             with pytest.raises(ValueError, match="cuda:1"):
                 calls[i]()
+
+
+def test_buffers_are_filled_before_a_constructor_returns(gsv, monkeypatch):
+    from gsv_b200 import quant
+
+    waited = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: types.SimpleNamespace(synchronize=lambda: waited.append(1)))
+    monkeypatch.setattr(quant, "_device_for", lambda device: torch.device("cpu"))
+    gsv.KVPlan(2, 4, 16, 8, 8)
+    gsv.KV4Workspace(2, 2, 2, 2, 32)
+    assert len(waited) == 2
+
+
+@pytest.mark.gpu
+def test_new_buffers_serve_another_stream(dev):
+    """Made behind queued work of the current stream, used at once on another one."""
+    other = torch.cuda.Stream()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = torch.randn(512, 4, 64, device="cuda").half()
+    cache, slots = dev.KV4Cache.empty(64, 16, 4, 64), torch.arange(512, device="cuda")
+    cache.append(rows, rows, slots)
+    table, q_start, kv_len = torch.arange(32, dtype=torch.int32, device="cuda")[None], i32(0, 512), i32(512)
+    state = (i32(0), i32(512), i32(*range(32))[None], i32(*range(64)), i32(64))
+    out = [torch.empty_like(rows) for _ in range(2)]
+    torch.cuda.synchronize()
+    cache.attention(rows, q_start, kv_len, table, 0.1, 512, dev.KV4Workspace(1, 512, 4, 4, 64), out=out[0])
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)  # some 50 ms
+    ws, plan = dev.KV4Workspace(1, 512, 4, 4, 64), dev.KVPlan(1, 32, 16, 64, 512)
+    cache.attention(rows, q_start, kv_len, table, 0.1, 512, ws, out=out[1], stream=other)
+    plan.run(*state, stream=other)
+    other.synchronize()
+    assert torch.equal(out[0], out[1])
+    assert plan.q_start.tolist() == [0, 512] and plan.slots.tolist() == [(63 - i // 16) * 16 + i % 16 for i in range(512)]
