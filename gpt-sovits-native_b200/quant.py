@@ -185,6 +185,14 @@ def _allocator(stream):
     return empty
 
 
+def _hold(stream, *tensors):
+    """Memory that a call on a stream that is given uses is its owner's to give
+    up at once, and the allocator's to keep until the call has run."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
 def _filled():
     """Waits for the fills of an object's own buffers, which calls on any stream
     may then use: the caller has no other handle on them.  (A capture orders
@@ -251,6 +259,9 @@ class KVPlan:
         a.kv_len = a.ctx_len if in_place else self.kv_len.data_ptr()
         a.free_left = a.free_count if in_place else self.free_left.data_ptr()
         check(lib().gsvk_kv_plan(byref(a), _stream_for(stream, here)))
+        if stream is not None:
+            _hold(stream, ctx_len, new_len, block_table, free_pages, free_count, self.q_start,
+                  self.kv_len, self.slots, self.free_left, self.refused, self._ticket)
         return self
 
     def release(self, done, length, block_table, free_pages, free_count, stream=None):
@@ -261,6 +272,8 @@ class KVPlan:
         check(lib().gsvk_kv_release(self.n_seq, self.max_blocks, self.n_pages, self.page_size,
                                     _vector(done, torch.int32, self.n_seq, "done", here), ln, table,
                                     free, count, _stream_for(stream, here)))
+        if stream is not None:
+            _hold(stream, done, length, block_table, free_pages, free_count)
 
 
 # ------------------------------------------------------------- 4-bit KV cache
@@ -315,8 +328,8 @@ class KV4Cache:
         import torch
 
         size = kv4_page_bytes(page_size, kv_heads, head_dim)
-        return cls(torch.empty(n_pages, max(size, 1), dtype=torch.uint8, device=_device_for(device)),
-                   page_size, kv_heads, head_dim)
+        pages = torch.empty(n_pages, max(size, 1), dtype=torch.uint8, device=_device_for(device))
+        return cls(pages, page_size, kv_heads, head_dim)
 
     def append(self, k, v, slots, stream=None):
         """Quantises rows [tokens, kv_heads, head_dim] (fp16 or fp32) into their
@@ -334,6 +347,8 @@ class KV4Cache:
         check(lib().gsvk_kv4_append(self._ref, kp, ks, vp, vs, dtype is torch.float32,
                                     _vector(slots, torch.int64, n, "slots", here), n,
                                     _stream_for(stream, here)))
+        if stream is not None:
+            _hold(stream, k, v, slots, self.pages)
 
     def read(self, slots, k=None, v=None, stream=None):
         """What the slots stand for: fp16 rows k and v [len(slots), kv_heads,
@@ -356,6 +371,8 @@ class KV4Cache:
         if v is not None:
             vp, vs = _rows(v, torch.float16, self.kv_heads, self.head_dim, "v", here)
         check(lib().gsvk_kv4_read(self._ref, sp, n, kp, ks, vp, vs, _stream_for(stream, here)))
+        if stream is not None:
+            _hold(stream, slots, k, v, self.pages)
         return k, v
 
     def attention(self, q, q_start, kv_len, block_table, scale: float, max_q: int, workspace,
@@ -389,9 +406,13 @@ class KV4Cache:
         a.prefix = None if prefix is None else _vector(prefix, i32, n_seq, "prefix", here)
         a.block_table = _vector(block_table, i32, 0, "block_table", here)
         if workspace.index != here:
-            raise ValueError(f"workspace: on cuda:{workspace.index}, the current device is cuda:{here}")
+            raise ValueError(f"workspace: on cuda:{workspace.index}, the current device is "
+                             f"cuda:{here}")
         a.workspace, a.workspace_bytes = workspace.ptr, workspace.bytes
         check(lib().gsvk_kv4_attention(self._attn_ref, _stream_for(stream, here)))
+        if stream is not None:
+            _hold(stream, q, q_start, kv_len, prefix, block_table, out, workspace.buffer,
+                  self.pages)
         return out
 
 
@@ -423,8 +444,11 @@ def quantize_rows_i8(x, q=None, scale=None, stream=None):
         sp = scale.data_ptr()
     else:
         sp = _vector(scale, torch.float32, rows, "scale", here)
-    check(lib().gsvk_quantize_rows_i8(xp, dtype is torch.float32, rows, n, _row_stride(x, rows, n, "x"), qp, ldq,
-                                      sp, _stream_for(stream, here)))
+    check(lib().gsvk_quantize_rows_i8(xp, dtype is torch.float32, rows, n,
+                                      _row_stride(x, rows, n, "x"), qp, ldq, sp,
+                                      _stream_for(stream, here)))
+    if stream is not None:
+        _hold(stream, x, q, scale)
     return q, scale
 
 
@@ -454,9 +478,11 @@ def gemm_i8(a, a_scale, b, b_scale, bias=None, residual=None, act=ACT_NONE, slop
     g = GemmI8Args(ap, _row_stride(a, M, K, "a"), bp, _row_stride(b, N, K, "b"),
                    _vector(a_scale, f32, M, "a_scale", here),
                    _vector(b_scale, f32, N, "b_scale", here), M, N, K,
-                   None if bias is None else _vector(bias, f32, N, "bias", here), rp, ldr, cp, ldc, hp,
-                   ldh, act, slope)
+                   None if bias is None else _vector(bias, f32, N, "bias", here), rp, ldr, cp,
+                   ldc, hp, ldh, act, slope)
     check(lib().gsvk_gemm_i8(byref(g), _stream_for(stream, here)))
+    if stream is not None:
+        _hold(stream, a, a_scale, b, b_scale, bias, residual, c, c_f16)
     return c if c is not None else c_f16
 
 

@@ -175,3 +175,47 @@ def test_new_buffers_serve_another_stream(dev):
     other.synchronize()
     assert torch.equal(out[0], out[1])
     assert plan.q_start.tolist() == [0, 512] and plan.slots.tolist() == [(63 - i // 16) * 16 + i % 16 for i in range(512)]
+
+
+@pytest.mark.gpu
+def test_memory_of_a_call_on_another_stream_is_kept_until_it_has_run(dev):
+    """Inputs that are given up while the call is still queued: their memory goes to nobody before it has run."""
+    other = torch.cuda.Stream()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    n = 1024
+    table, q_start, kv_len = torch.arange(64, dtype=torch.int32, device="cuda")[None], i32(0, n), i32(n)
+    slots = torch.arange(n, device="cuda")
+    rows = lambda: torch.ones(n, 4, 128, dtype=torch.float16, device="cuda")  # noqa: E731
+    codes = lambda: torch.ones(n, 1024, dtype=torch.int8, device="cuda")  # noqa: E731
+    cache = dev.KV4Cache.empty(64, 16, 4, 128)
+    space = dev.KV4Workspace(1, n, 4, 4, 128)
+    one, out, i8 = torch.ones(n, device="cuda"), rows(), codes()
+
+    def quantise(x):
+        dev.quantize_rows_i8(x, stream=other)
+
+    def attention(q):
+        cache.attention(q, q_start, kv_len, table, 0.1, n, space, out=out, stream=other)
+
+    makes = ((lambda: torch.ones(n, 1024, device="cuda"), quantise), (rows, attention),
+             (codes, lambda a: dev.gemm_i8(a, one, i8, one, stream=other)),
+             (codes, lambda b: dev.gemm_i8(i8, one, b, one, stream=other)),
+             (rows, lambda k: cache.append(k, out, slots, stream=other)),
+             (lambda: torch.empty(1 << 20, dtype=torch.int64, device="cuda").fill_(-1), lambda s: cache.read(s, k=out_wide, stream=other)),
+             (lambda: dev.KV4Cache.empty(256, 16, 4, 128), lambda c: c.append(out, out, slots, stream=other)),
+             (lambda: dev.KV4Workspace(1, n, 4, 4, 128), lambda ws: cache.attention(out, q_start, kv_len, table, 0.1, n, ws, out=out,
+                                                                                  stream=other)))
+    out_wide = torch.empty(1 << 20, 4, 128, dtype=torch.float16, device="cuda")
+    cache.append(out, out, slots)
+    for make, call in makes:
+        given = make()
+        t = given.pages if isinstance(given, dev.KV4Cache) else given.buffer if isinstance(given, dev.KV4Workspace) else given
+        shape, dtype, at = t.shape, t.dtype, t.data_ptr()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(20_000_000)  # some 10 ms
+        call(given)
+        del given, t
+        again = torch.empty(shape, dtype=dtype, device="cuda")
+        assert again.data_ptr() != at
+        other.synchronize()
