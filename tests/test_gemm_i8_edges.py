@@ -106,3 +106,22 @@ def test_more_outputs_than_a_launch_holds_are_refused(gsv, M, N):
     for ld in (64, 65):
         g = GemmI8Args(a=256, lda=ld, b=256, ldb=ld, a_scale=256, b_scale=256, M=M, N=N, K=64, c=256, ldc=N)
         assert gsv.lib().gsvk_gemm_i8(ctypes.byref(g), None) == -5
+
+
+def test_the_packed_gelu_has_gelu_erfs_constants():
+    """The polynomial of Phi(-u) stands in both sources, two values to an operation in the product's: the same numbers."""
+    import os
+    import re
+
+    src = os.path.join(os.path.dirname(__file__), "..", "gpt-sovits-native_b200", "csrc")
+
+    def body(name, start):
+        text = open(os.path.join(src, name)).read()
+        text = text[text.index(start):]
+        return text[:text.index("\n}\n")]
+
+    scalar = re.findall(r"[-+]?\d\.\d+e[-+]\d+f", body("common.cuh", "float gelu_erf(float x)"))
+    packed = re.findall(r"pair\(([-+]?\d\.\d+e[-+]\d+f), ([-+]?\d\.\d+e[-+]\d+f)\)", body("gemm_i8.cu", "void gelu2("))
+    assert len(scalar) == 11 and packed == [(c, c) for c in scalar]
+    for text in (body("common.cuh", "float gelu_erf(float x)"), body("gemm_i8.cu", "void gelu2(")):
+        assert "-0.721347520444f" in text and "5.5f" in text
